@@ -1,0 +1,420 @@
+// Gradients of window attention (window_attn_fwd.hip) for f16 / bf16 / float32 on the matrix cores.
+//
+//     P = exp(scale Q K^T - lse) where seen, else 0          dV = P^T dO
+//     dP = dO V^T,  delta = rowsum(dO o O),  dS = P o (dP - delta)
+//     dQ = scale dS K,   dK = scale dS^T Q                   dK, dV summed over the query heads that share them
+//
+// Three kernels and, where keys are split, a fourth; no atomics, so results do not depend on timing.
+//   rows    per query row: -delta and lse * log2(e), in float32, in an array padded to whole tiles whose
+//           padding and whose rows that see nothing get lse = +inf (P = 0).
+//   dQ      workgroup = 128 query rows (4 waves x 32) and the key tiles they see, as in the forward:
+//           S^T = K Q^T and dP^T = V dO^T put the query on the lane; dS^T is in place the B operand of
+//           dQ^T += K^T dS^T.
+//   dK, dV  workgroup = 128 keys (4 waves x 32) of one key/value head and, head after head of its group,
+//           the query tiles that see some of them: S = Q K^T and dP = dO V^T put the key on the lane; P and
+//           dS are in place the B operands of dV^T += dO^T P and dK^T += Q^T dS.  The sums over the group
+//           happen in the accumulators.
+//   join    The first `sinks` keys are seen by every later query, the others by about `window`: key blocks
+//           with sinks are split over several workgroups by queries, their float32 parts added here in order.
+// Beyond 128 columns a workgroup of dK, dV keeps 128 columns of both (the accumulators and the fragments of
+// its keys fill the registers) and forms S and dP for each half again.
+// P and dS are rounded to the element type as operands; everything else is float32.  Rows and keys that
+// have no visible partner in the workgroup are fetched as zeros, so whatever stands there stays out.
+#include "window_attn_common.h"
+
+namespace myfa {
+namespace {
+
+template <typename T, int D> constexpr int bwd_tile() { return D * (int)sizeof(T) <= 256 ? 64 : 32; }
+constexpr int kStatPad = 64;                         // rows of the statistics per head: a multiple of this
+
+// ---------------------------------------------------------------- row statistics
+template <typename T>
+__global__ void __launch_bounds__(256)
+window_bwd_rows_kernel(const T* __restrict__ Og, const T* __restrict__ dOg, const float* __restrict__ LSEg,
+                       float* __restrict__ st, WindowShape w, int nqp, int64_t rows) {
+    constexpr int EPC = 16 / (int)sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(EPC)));
+    const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);     // padded row
+    if (row >= rows) return;
+    const int64_t bh = row / nqp;
+    const int i = (int)(row - bh * nqp), b = (int)(bh / w.H);
+    const int len = w.lens ? w.lens[b] : w.Nk;
+    const bool live = i < w.Nq && i + w.Nk - w.Nq < len;
+    float acc = 0.f;
+    if (live) {
+        const int64_t at = (bh * w.Nq + i) * w.d;
+        for (int c = (threadIdx.x & 15) * EPC; c < w.d; c += 16 * EPC) {
+            const vec x = *reinterpret_cast<const vec*>(Og + at + c), y = *reinterpret_cast<const vec*>(dOg + at + c);
+#pragma unroll
+            for (int j = 0; j < EPC; ++j) acc += (float)x[j] * (float)y[j];
+        }
+    }
+    acc += dpp_mov<0xB1>(acc);
+    acc += dpp_mov<0x4E>(acc);
+    acc += dpp_mov<0x141>(acc);
+    acc += dpp_mov<0x140>(acc);
+    if ((threadIdx.x & 15) == 0) {
+        st[row] = live ? LSEg[bh * w.Nq + i] * kLog2eW : INFINITY;
+        st[rows + row] = live ? -acc : 0.f;
+    }
+}
+
+// ---------------------------------------------------------------- dQ
+template <typename T, int D>
+__global__ void __launch_bounds__(256, D * sizeof(T) <= 256 ? 2 : 1)
+window_bwd_dq_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
+                     const T* __restrict__ dOg, const float* __restrict__ st, T* __restrict__ dQg,
+                     WindowShape w, int nqp, int64_t rows, int nqblk, int nwg) {
+    using R = TileReader<T, D>;
+    constexpr int BN = bwd_tile<T, D>(), NB = BN / 32, TILE_B = BN * R::RB;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B];   // K0 K1 V0 V1
+
+    const int lid = xcd_range_id(blockIdx.x, nwg);
+    const int bh = lid / nqblk;
+    const int b = bh / w.H, head = bh - b * w.H, kvh = head / (w.H / w.Hkv);
+    const int q0 = (lid - bh * nqblk) * 128;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5;
+    const int len = w.lens ? min(max(w.lens[b], 0), w.Nk) : w.Nk;
+    const int shift = w.Nk - w.Nq;
+    const int pa = q0 + shift, pz = min(min(q0 + 128, w.Nq) + shift, len);
+    const int lo = max(0, pa - w.window + 1);
+    const int t_win = lo / BN, t_end = pz > pa ? (pz + BN - 1) / BN : t_win;
+    const int n_sink = pz > pa ? min((min(w.sinks, pz) + BN - 1) / BN, t_win) : 0;
+    const int ntiles = n_sink + (t_end - t_win);
+
+    const int qrow = q0 + 32 * wave + r;
+    const int p_own = qrow + shift;
+    const bool live = qrow < w.Nq && p_own < len;
+    const int p_hi = live ? p_own : -1, p_lo = p_own - w.window + 1;
+    const int wave_lo = q0 + 32 * wave + shift, wave_hi = min(wave_lo + 32, pz) - 1;
+
+    const T* Kh = Kg + b * w.ks[0] + kvh * w.ks[1];
+    const T* Vh = Vg + b * w.vs[0] + kvh * w.vs[1];
+    constexpr int EPC = 16 / (int)sizeof(T);
+    typename R::frag qf[R::KS], of[R::KS];
+    {
+        const int row = min(qrow, w.Nq - 1);
+        const T* qp = Qg + b * w.qs[0] + head * w.qs[1] + (int64_t)row * w.qs[2];
+        const T* op = dOg + ((int64_t)bh * w.Nq + row) * w.d;
+#pragma unroll
+        for (int ks = 0; ks < R::KS; ++ks) {
+            const int c = (2 * ks + h) * EPC;
+            qf[ks] = typename R::frag{};
+            of[ks] = typename R::frag{};
+            if (c < w.d) {
+                qf[ks] = *reinterpret_cast<const typename R::frag*>(qp + c);
+                of[ks] = *reinterpret_cast<const typename R::frag*>(op + c);
+            }
+        }
+    }
+    const int64_t srow = (int64_t)bh * nqp + min(qrow, nqp - 1);
+    const float lse2 = st[srow], ndelta = st[rows + srow];
+    const float sl2 = w.scale * kLog2eW;
+
+    const R rd(lane);
+    const TileFetch<T, D, BN, 256> kfetch(tid, w.ks[2], w.d), vfetch(tid, w.vs[2], w.d);
+    auto first_key = [&](int t) __attribute__((always_inline)) { return (t < n_sink ? t : t - n_sink + t_win) * BN; };
+    auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
+        const int k0 = first_key(t);
+        const bool all = k0 + BN <= pz && (k0 >= lo || k0 + BN <= w.sinks);
+        auto keep = [&](int row) { const int k = k0 + row; return (k < pz) & ((k >= lo) | (k < w.sinks)); };
+        kfetch.fetch(Kh + (int64_t)k0 * w.ks[2], lds + buf * TILE_B, all, keep);
+        vfetch.fetch(Vh + (int64_t)k0 * w.vs[2], lds + (2 + buf) * TILE_B, all, keep);
+    };
+
+    f32x16 dq[R::DB];
+#pragma unroll
+    for (int db = 0; db < R::DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dq[db][i] = 0.f;
+
+    if (ntiles > 0) fetch(0, 0);
+    for (int t = 0; t < ntiles; ++t) {
+        const int buf = t & 1, k0 = first_key(t);
+        tile_ready();
+        if (t + 1 < ntiles) fetch(t + 1, buf ^ 1);
+        if (k0 > wave_hi || (k0 + BN <= wave_lo - w.window + 1 && k0 >= w.sinks)) continue;
+        const char* Kb = lds + buf * TILE_B;
+        const char* Vb = lds + (2 + buf) * TILE_B;
+        const bool edge = !(k0 + BN - 1 <= wave_lo && wave_lo + 31 < len && wave_lo + 31 - shift < w.Nq &&
+                            (k0 >= wave_lo + 31 - w.window + 1 || k0 + BN <= w.sinks));
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb) {
+            f32x16 s, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = ndelta; }
+#pragma unroll
+            for (int ks = 0; ks < R::KS; ++ks) s = mma_chunk<T>(rd.row(Kb, kb, ks), qf[ks], s);
+#pragma unroll
+            for (int ks = 0; ks < R::KS; ++ks) dp = mma_chunk<T>(rd.row(Vb, kb, ks), of[ks], dp);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sl2, -lse2)) * dp[i];
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = k0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
+                    if (!((key <= p_hi) & ((key >= p_lo) | (key < w.sinks)))) s[i] = 0.f;
+                }
+            }
+            rd.add_transposed(Kb, kb, s, dq);
+        }
+    }
+
+    if (qrow < w.Nq) {
+        T* row = dQg + ((int64_t)bh * w.Nq + qrow) * w.d;
+        typedef T vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (int db = 0; db < R::DB; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = 32 * db + 8 * g + 4 * h;
+                vec4 x;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = live ? (T)(dq[db][4 * g + j] * w.scale) : (T)0.f;
+                if (c < w.d) *reinterpret_cast<vec4*>(row + c) = x;
+            }
+    }
+}
+
+// ---------------------------------------------------------------- dK, dV
+template <typename T, int D>
+__global__ void __launch_bounds__(256, D * sizeof(T) <= 128 ? 2 : 1)
+window_bwd_dkv_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
+                      const T* __restrict__ dOg, const float* __restrict__ st, T* __restrict__ dKg, T* __restrict__ dVg,
+                      float* __restrict__ parts, WindowShape w, int nqp, int64_t rows, int nkblk, int nsb, int ns, int nwg) {
+    using R = TileReader<T, D>;
+    constexpr int BQ = bwd_tile<T, D>(), NB = BQ / 32, TILE_B = BQ * R::RB;
+    constexpr int ODB = R::DB < 4 ? R::DB : 4, NC = R::DB / ODB;             // column blocks kept, workgroups per key block
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B + 4 * 64 * 4];   // Q0 Q1 dO0 dO1 [buf][lse2 | -delta][64]
+    float* stat = reinterpret_cast<float*>(lds + 4 * TILE_B);
+
+    // a head's units: the split sink blocks first (the longest), then the other key blocks
+    const int units = nsb * ns + (nkblk - nsb);
+    const int lidc = xcd_range_id(blockIdx.x, nwg), lid = lidc / NC, col0 = (lidc - lid * NC) * ODB * 32;
+    const int bg = lid / units, unit = lid - bg * units;
+    const bool split = unit < nsb * ns;
+    const int kblk = split ? unit / ns : unit - nsb * ns + nsb, part = split ? unit - kblk * ns : 0, nparts = split ? ns : 1;
+    const int b = bg / w.Hkv, kvh = bg - b * w.Hkv, group = w.H / w.Hkv;
+    const int k0 = kblk * 128;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5;
+    const int len = w.lens ? min(max(w.lens[b], 0), w.Nk) : w.Nk;
+    const int shift = w.Nk - w.Nq;
+    // positions that see some key of the block: [pa, pz)
+    const int pa = max(k0, shift), pz = k0 < w.sinks ? len : min(len, k0 + 127 + w.window);
+    const int tq0 = (pa - shift) / BQ, nt = pz > pa ? (pz - shift + BQ - 1) / BQ - tq0 : 0;
+    const int total = nt * group;
+    const int j0 = (int)((int64_t)total * part / nparts), j1 = (int)((int64_t)total * (part + 1) / nparts);
+
+    const int krow = k0 + 32 * wave + r;
+    // positions that see the lane's key
+    const int p_lo = krow, p_hi = krow >= w.Nk ? -1 : krow < w.sinks ? len - 1 : min(len - 1, krow + w.window - 1);
+    const int key_a = k0 + 32 * wave, key_z = key_a + 31;                 // the wave's keys
+
+    constexpr int EPC = 16 / (int)sizeof(T);
+    typename R::frag kf[R::KS], vf[R::KS];
+    {
+        const int row = min(krow, w.Nk - 1);
+        const T* kp = Kg + b * w.ks[0] + kvh * w.ks[1] + (int64_t)row * w.ks[2];
+        const T* vp = Vg + b * w.vs[0] + kvh * w.vs[1] + (int64_t)row * w.vs[2];
+#pragma unroll
+        for (int ks = 0; ks < R::KS; ++ks) {
+            const int c = (2 * ks + h) * EPC;
+            kf[ks] = typename R::frag{};
+            vf[ks] = typename R::frag{};
+            if (c < w.d) {
+                kf[ks] = *reinterpret_cast<const typename R::frag*>(kp + c);
+                vf[ks] = *reinterpret_cast<const typename R::frag*>(vp + c);
+            }
+        }
+    }
+    const float sl2 = w.scale * kLog2eW;
+
+    const R rd(lane);
+    const TileFetch<T, D, BQ, 256> qfetch(tid, w.qs[2], w.d), ofetch(tid, w.d, w.d);
+    auto fetch = [&](int j, int buf) __attribute__((always_inline)) {
+        const int g = j / nt, i0 = (tq0 + j - g * nt) * BQ;
+        const int head = kvh * group + g;
+        const int64_t bh = (int64_t)b * w.H + head;
+        const bool all = i0 + shift >= pa && i0 + BQ + shift <= pz;
+        auto keep = [&](int row) { const int p = i0 + row + shift; return (p >= pa) & (p < pz); };
+        qfetch.fetch(Qg + b * w.qs[0] + head * w.qs[1] + (int64_t)i0 * w.qs[2], lds + buf * TILE_B, all, keep);
+        ofetch.fetch(dOg + (bh * w.Nq + i0) * w.d, lds + (2 + buf) * TILE_B, all, keep);
+#if defined(__HIP_DEVICE_COMPILE__)
+        if (wave < 2) {
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(st + wave * rows + bh * nqp + i0), 0, BQ * 4, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(stat + (2 * buf + wave) * 64), 4, lane * 4, 0, 0, 0);
+        }
+#endif
+    };
+
+    f32x16 dk[ODB], dv[ODB];
+#pragma unroll
+    for (int db = 0; db < ODB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { dk[db][i] = 0.f; dv[db][i] = 0.f; }
+
+    if (j0 < j1) fetch(j0, 0);
+    for (int j = j0; j < j1; ++j) {
+        const int buf = (j - j0) & 1;
+        tile_ready();
+        if (j + 1 < j1) fetch(j + 1, buf ^ 1);
+        const int g = j / nt, pt = (tq0 + j - g * nt) * BQ + shift;              // position of the tile's first row
+        if (pt + BQ <= key_a || (key_a >= w.sinks && pt > key_z + w.window - 1)) continue;
+        const char* Qb = lds + buf * TILE_B;
+        const char* Ob = lds + (2 + buf) * TILE_B;
+        const float* lse2b = stat + 2 * buf * 64;
+        const bool edge = !(pt >= key_z && pt + BQ <= len && key_z < w.Nk && (key_z < w.sinks || pt + BQ - 1 < key_a + w.window));
+#pragma unroll
+        for (int qb = 0; qb < NB; ++qb) {
+            f32x16 s, dp;
+            f32x4 l4[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                l4[q] = *reinterpret_cast<const f32x4*>(lse2b + 32 * qb + 8 * q + 4 * h);
+                const f32x4 nd = *reinterpret_cast<const f32x4*>(lse2b + 64 + 32 * qb + 8 * q + 4 * h);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { s[4 * q + e] = 0.f; dp[4 * q + e] = nd[e]; }
+            }
+#pragma unroll
+            for (int ks = 0; ks < R::KS; ++ks) s = mma_chunk<T>(rd.row(Qb, qb, ks), kf[ks], s);
+#pragma unroll
+            for (int ks = 0; ks < R::KS; ++ks) dp = mma_chunk<T>(rd.row(Ob, qb, ks), vf[ks], dp);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sl2, -l4[i >> 2][i & 3]));
+                dp[i] *= s[i];
+            }
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int p = pt + 32 * qb + 8 * (i >> 2) + 4 * h + (i & 3);
+                    if ((p < p_lo) | (p > p_hi)) { s[i] = 0.f; dp[i] = 0.f; }
+                }
+            }
+            rd.add_transposed(Ob + R::COLB * (col0 / 32), qb, s, dv);
+            rd.add_transposed(Qb + R::COLB * (col0 / 32), qb, dp, dk);
+        }
+    }
+
+    if (krow >= w.Nk) return;
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    const int64_t at = ((int64_t)bg * w.Nk + krow) * w.d;
+    float* pk = parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 + (krow - k0)) * w.d;
+#pragma unroll
+    for (int db = 0; db < ODB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = col0 + 32 * db + 8 * g + 4 * h;
+            if (c >= w.d) continue;
+            f32x4 xk, xv;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { xk[e] = dk[db][4 * g + e] * w.scale; xv[e] = dv[db][4 * g + e]; }
+            if (split && ns > 1) {
+                *reinterpret_cast<f32x4*>(pk + c) = xk;
+                *reinterpret_cast<f32x4*>(pk + (int64_t)128 * w.d + c) = xv;
+            } else {
+                vec4 yk, yv;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { yk[e] = (T)xk[e]; yv[e] = (T)xv[e]; }
+                *reinterpret_cast<vec4*>(dKg + at + c) = yk;
+                *reinterpret_cast<vec4*>(dVg + at + c) = yv;
+            }
+        }
+}
+
+// ---------------------------------------------------------------- the split key blocks' parts, in order
+template <typename T>
+__global__ void __launch_bounds__(256)
+window_bwd_join_kernel(const float* __restrict__ parts, T* __restrict__ dKg, T* __restrict__ dVg, int Nk, int d, int nsb, int ns, int64_t n4) {
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (u >= n4) return;
+    const int per_row = d / 4;
+    const int c = (int)(u % per_row) * 4;
+    int64_t x = u / per_row;
+    const int row = (int)(x % 128); x /= 128;
+    const int which = (int)(x % 2); x /= 2;
+    const int kblk = (int)(x % nsb);
+    const int64_t bg = x / nsb;
+    const int krow = kblk * 128 + row;
+    if (krow >= Nk) return;
+    const float* p = parts + (((bg * nsb + kblk) * ns * 2 + which) * 128 + row) * (int64_t)d + c;
+    f32x4 sum = *reinterpret_cast<const f32x4*>(p);
+    for (int i = 1; i < ns; ++i) sum += *reinterpret_cast<const f32x4*>(p + (int64_t)i * 2 * 128 * d);
+    vec4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = (T)sum[e];
+    *reinterpret_cast<vec4*>((which ? dVg : dKg) + (bg * Nk + krow) * (int64_t)d + c) = y;
+}
+
+// ---------------------------------------------------------------- host
+struct BwdPlan { int nqp, nkblk, nsb, ns; int64_t rows, stat_floats, part_floats; };
+
+// How many workgroups share a key block with sinks: enough that none has more than about a plain block's
+// queries, at most 32 (the parts are written and read once more).
+BwdPlan bwd_plan(const WindowShape& w) {
+    BwdPlan p;
+    p.nqp = (int)cdiv(w.Nq, kStatPad) * kStatPad;
+    p.rows = (int64_t)w.B * w.H * p.nqp;
+    p.nkblk = (int)cdiv(w.Nk, 128);
+    const bool uneven = w.sinks > 0 && w.window + 128 < w.Nk;
+    p.nsb = uneven ? (int)cdiv(w.sinks, 128) : 0;
+    const int64_t each = cdiv(w.Nk, (int64_t)w.window + 128);
+    p.ns = p.nsb > 0 ? (int)(each < 32 ? each : 32) : 1;
+    p.stat_floats = 2 * p.rows;
+    p.part_floats = p.ns > 1 ? (int64_t)w.B * w.Hkv * p.nsb * p.ns * 2 * 128 * w.d : 0;
+    return p;
+}
+
+template <typename T>
+int launch_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
+               void* dq, void* dk, void* dv, float* ws, const WindowShape& w, hipStream_t s) {
+    const BwdPlan p = bwd_plan(w);
+    float* st = ws;
+    float* parts = ws + p.stat_floats;
+    const int nqblk = (int)cdiv(w.Nq, 128);
+    const int64_t nq = (int64_t)w.B * w.H * nqblk, nkv = (int64_t)w.B * w.Hkv * (p.nsb * (int64_t)p.ns + p.nkblk - p.nsb) * (w.d > 128 ? 2 : 1);
+    if (nq > 0x7fffffff || nkv > 0x7fffffff || cdiv(p.rows, 16) > 0x7fffffff)
+        return fail(MYFA_E_UNSUPPORTED, "window attention backward: too many blocks");
+    if (p.rows > 0)
+        launch_kernel(window_bwd_rows_kernel<T>, dim3((unsigned)cdiv(p.rows, 16)), dim3(256), 0, s, static_cast<const T*>(o),
+                      static_cast<const T*>(dout), lse, st, w, p.nqp, p.rows);
+    auto go = [&](auto kdq, auto kdkv) {
+        launch_kernel(kdkv, dim3((unsigned)nkv), dim3(256), 0, s, static_cast<const T*>(q), static_cast<const T*>(k),
+                      static_cast<const T*>(v), static_cast<const T*>(dout), st, static_cast<T*>(dk), static_cast<T*>(dv), parts,
+                      w, p.nqp, p.rows, p.nkblk, p.nsb, p.ns, (int)nkv);
+        if (nq > 0)
+            launch_kernel(kdq, dim3((unsigned)nq), dim3(256), 0, s, static_cast<const T*>(q), static_cast<const T*>(k),
+                          static_cast<const T*>(v), static_cast<const T*>(dout), st, static_cast<T*>(dq), w, p.nqp, p.rows, nqblk, (int)nq);
+    };
+    if (w.d <= 64) go(window_bwd_dq_kernel<T, 64>, window_bwd_dkv_kernel<T, 64>);
+    else if (w.d <= 128) go(window_bwd_dq_kernel<T, 128>, window_bwd_dkv_kernel<T, 128>);
+    else if constexpr (sizeof(T) == 2) go(window_bwd_dq_kernel<T, 256>, window_bwd_dkv_kernel<T, 256>);
+    if (p.ns > 1) {
+        const int64_t n4 = (int64_t)w.B * w.Hkv * p.nsb * 2 * 128 * (w.d / 4);
+        launch_kernel(window_bwd_join_kernel<T>, dim3((unsigned)cdiv(n4, 256)), dim3(256), 0, s, parts, static_cast<T*>(dk),
+                      static_cast<T*>(dv), w.Nk, w.d, p.nsb, p.ns, n4);
+    }
+    return check_launch("window attention backward");
+}
+
+}  // namespace
+
+int64_t window_attn_bwd_ws_bytes(const WindowShape& w) {
+    const BwdPlan p = bwd_plan(w);
+    return (p.stat_floats + p.part_floats) * 4;
+}
+
+int window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
+                    void* dq, void* dk, void* dv, float* ws, const WindowShape& w, int dtype, hipStream_t s) {
+    if (dtype == MYFA_F32) return launch_bwd<float>(q, k, v, o, lse, dout, dq, dk, dv, ws, w, s);
+    if (dtype == MYFA_F16) return launch_bwd<_Float16>(q, k, v, o, lse, dout, dq, dk, dv, ws, w, s);
+    return launch_bwd<__bf16>(q, k, v, o, lse, dout, dq, dk, dv, ws, w, s);
+}
+
+}  // namespace myfa

@@ -1,0 +1,161 @@
+// Pieces shared by the window attention kernels (forward and backward): the shape record, what a query
+// sees, and the products of a 32-row block with an LDS tile, for 16-bit and float32 elements alike.
+//
+// What a query sees.  Query i of a sequence stands at position p = i + Nk - Nq.  It sees key j when
+//     j <= p  and  p < len  and  ( p - j < window  or  j < sinks ),
+// len being the sequence's length (Nk where the caller gives none).  A position p >= len sees nothing.
+//
+// Fragments.  Both element types move through the matrix cores in 16-byte chunks: a lane's chunk is the
+// A or B operand of one v_mfma_f32_32x32x16 (16-bit) or of four v_mfma_f32_32x32x2_f32, one per element,
+// where the two lane halves hold chunk 2s and 2s + 1 of the row, i.e. the k index of MFMA e of step s is
+// column 8s + 4h + e on both operands.  The accumulator layout is the same: lane (r = l & 31, h = l >> 5)
+// holds column r and rows 8 (i >> 2) + 4 h + (i & 3), i = 0..15.
+#ifndef MYFA_WINDOW_ATTN_COMMON_H_
+#define MYFA_WINDOW_ATTN_COMMON_H_
+#include "attn_mfma_common.h"
+
+namespace myfa {
+
+struct WindowShape {
+    int B, H, Hkv, Nq, Nk, d;
+    int window, sinks;                 // both clamped to Nk
+    float scale;
+    const int* lens;                   // [B] or null
+    int64_t qs[3], ks[3], vs[3];       // strides of batch, head, row, in elements
+};
+
+namespace {
+
+constexpr float kLog2eW = 1.4426950408889634f;
+constexpr float kLn2W = 0.6931471805599453f;
+// Fetches of rows or columns that are not there use this offset: behind every buffer's end, answered
+// with zeros without touching memory.  In-tile offsets stay below kTileBytesMax (checked by the host).
+constexpr int kOffPast = 0x7FFF0000;
+constexpr int kTileBytesMax = 0x7FFE0000;
+
+template <typename T> struct Frag16 { using type = s16x8; };
+template <> struct Frag16<float> { using type = f32x4; };
+
+// c += a b over one 16-byte chunk per lane
+template <typename T>
+__device__ __forceinline__ f32x16 mma_chunk(typename Frag16<T>::type a, typename Frag16<T>::type b, f32x16 c) {
+    if constexpr (sizeof(T) == 2) {
+        return Mma<T>::run(a, __builtin_bit_cast(typename Mma<T>::vec8, b), c);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+}
+
+// The per-lane bases of the reads from a [rows][D] tile image (8-row x 64-byte subtiles, see img_off):
+// row chunks, and the transposed operand whose k index runs over the tile's rows.
+template <typename T, int D> struct TileReader {
+    static constexpr int RB = D * (int)sizeof(T);      // bytes of a row
+    static constexpr int SUB = 8 * RB;                 // bytes of 8 rows
+    static constexpr int KS = RB / 32;                 // chunk pairs of a row
+    static constexpr int DB = D / 32;
+    using frag = typename Frag16<T>::type;
+    int rb[2], tb[2];
+
+    __device__ __forceinline__ TileReader(int lane) {
+        const int r = lane & 31, h = lane >> 5;
+        const int tq = (lane & 15) >> 2, tp = lane & 3, tg1 = (lane >> 4) & 1;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            rb[e] = SUB * (r >> 3) + 64 * (r & 7) + 16 * ((2 * e + h) ^ ((r >> 2) & 3));
+            if constexpr (sizeof(T) == 2)
+                tb[e] = 64 * (4 * h + tq) + 16 * ((2 * tg1 + (tp >> 1)) ^ (2 * e + h)) + 8 * (tp & 1) + SUB * e;
+            else
+                tb[e] = 512 * (r >> 4) + 256 * h + 16 * (((r >> 2) & 3) ^ (2 * e + h)) + 4 * (r & 3);
+        }
+    }
+    // chunk 2 ks + h of row 32 blk + r
+    __device__ __forceinline__ frag row(const char* tile, int blk, int ks) const {
+        return *reinterpret_cast<const frag*>(tile + rb[ks & 1] + SUB * 4 * blk + 512 * (ks >> 1));
+    }
+    // acc[db] += tile[rows of blk][32 columns of db]^T x[rows of blk], x an accumulator-shaped block
+    // (rounded to T): the accumulator's row index is this product's k index, in place.  `tile` may point
+    // at a later column block (COLB bytes each): acc then holds the columns from there on.
+    static constexpr int COLB = sizeof(T) == 2 ? 512 : 1024;
+    template <int NDB>
+    __device__ __forceinline__ void add_transposed(const char* tile, int blk, const f32x16& x, f32x16 (&acc)[NDB]) const {
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                typename Mma<T>::vec8 b;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) b[j] = (T)x[8 * st + j];
+#pragma unroll
+                for (int db = 0; db < NDB; ++db) {
+                    const int imm = SUB * 2 * (2 * blk + st) + COLB * db;
+                    const s16x4 lo = lds_read_tr(tile + tb[0] + imm);
+                    const s16x4 hi = lds_read_tr(tile + tb[1] + imm);
+                    s16x8 a;
+                    a[0] = lo[0]; a[1] = lo[1]; a[2] = lo[2]; a[3] = lo[3];
+                    a[4] = hi[0]; a[5] = hi[1]; a[6] = hi[2]; a[7] = hi[3];
+                    acc[db] = Mma<T>::run(a, b, acc[db]);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+#pragma unroll
+                for (int db = 0; db < NDB; ++db) {
+                    const float a = *reinterpret_cast<const float*>(tile + tb[(i >> 2) & 1] + SUB * (4 * blk + (i >> 2)) +
+                                                                    COLB * db + 64 * (i & 3));
+                    acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x[i], acc[db], 0, 0, 0);
+                }
+        }
+    }
+};
+
+// Fetches [ROWS][D] tiles straight into LDS (one wave instruction fills 1 KiB of the image, so the image
+// is produced by choosing each lane's source chunk).  Columns from d on read as zeros.
+template <typename T, int D, int ROWS, int THREADS> struct TileFetch {
+    static constexpr int RB = D * (int)sizeof(T), CPR = RB / 16, LPT = ROWS * CPR / THREADS;
+    static_assert(LPT >= 1 && ROWS * CPR % THREADS == 0, "every thread fetches whole chunks");
+    int off[LPT], row[LPT];
+    int wave;
+    __device__ __forceinline__ TileFetch(int tid, int64_t row_stride, int d) : wave(__builtin_amdgcn_readfirstlane(tid >> 6)) {
+        const int lane = tid & 63;
+#pragma unroll
+        for (int i = 0; i < LPT; ++i) {
+            const int u = 64 * (wave * LPT + i) + lane;
+            const int grp8 = u / (RB / 2), within = u % (RB / 2);
+            row[i] = 8 * grp8 + ((within & 31) >> 2);
+            const int ch = 4 * (within >> 5) + ((within & 3) ^ ((row[i] >> 2) & 3));
+            off[i] = ch * (16 / (int)sizeof(T)) < d ? (row[i] * (int)row_stride + ch * (16 / (int)sizeof(T))) * (int)sizeof(T) : kOffPast;
+        }
+    }
+    // rows of the tile for which keep(row) does not hold read as zeros
+    template <class Keep>
+    __device__ __forceinline__ void fetch(const T* base, char* lds, bool all, Keep&& keep) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kTileBytesMax, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < LPT; ++i) {
+            const int o = (int)all | (int)keep(row[i]) ? off[i] : kOffPast;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(lds + 1024 * (wave * LPT + i)), 16, o, 0, 0, 0);
+        }
+#endif
+    }
+};
+
+// Everyone's fetches so far are complete and everyone has left the tile read before.
+__device__ __forceinline__ void tile_ready() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Consecutive logical ids share keys and values; every XCD (workgroup id mod 8) gets a contiguous range
+// of them, so that what they share stays in its L2.  Speed only.
+__device__ __forceinline__ int xcd_range_id(int bid, int n) {
+    const int xcd = bid & 7, idx = bid >> 3, q = n >> 3, rr = n & 7;
+    return (xcd < rr ? xcd * (q + 1) : rr * (q + 1) + (xcd - rr) * q) + idx;
+}
+
+}  // namespace
+}  // namespace myfa
+#endif  // MYFA_WINDOW_ATTN_COMMON_H_

@@ -11,6 +11,11 @@ plus the batched forward the reference sketches but never wrote
 
     flash_attn_fwd(q, k, v, scale=1.0, return_lse=False)     # (B, H, N, d)
 
+and what a decoder with a sliding window and a paged cache runs beside it (window.py, paged.py):
+
+    window_attn_fwd / window_attn_bwd / window_attn_func     sliding window + first tokens, grouped heads
+    paged_kv_append, paged_attn_decode, paged_kv_evict       fill a paged cache, read it, cut it
+
 The host side is Python: it validates arguments the way the reference's C++
 does (CHECK_INPUT = device tensor + contiguous, csrc/my_flash_attn/util.hpp:7-9;
 size checks, csrc/api.cpp:18,45,73,182-183; failures surface as RuntimeError,
@@ -26,7 +31,9 @@ from . import _lib
 from ._lib import MYFA_BF16, MYFA_F16, MYFA_F32, device_info  # noqa: F401
 
 __all__ = ["my_softmax", "my_attention", "my_matmul", "my_matmul_cublas", "my_matmul_out",
-           "flash_attn_fwd", "flash_attn_bwd", "flash_attn_bwd_into", "flash_attn_func", "softmax_rows", "softmax", "device_info"]
+           "flash_attn_fwd", "flash_attn_bwd", "flash_attn_bwd_into", "flash_attn_func", "softmax_rows", "softmax", "device_info",
+           "window_attn_fwd", "window_attn_bwd", "window_attn_func",
+           "paged_kv_append", "paged_attn_decode", "paged_kv_evict"]
 
 _DTYPE_TAG = {torch.float32: MYFA_F32, torch.float16: MYFA_F16, torch.bfloat16: MYFA_BF16}
 
@@ -39,6 +46,34 @@ def _check_input(x, name):
         raise RuntimeError(f"{name} must be a CUDA tensor")
     if not x.is_contiguous():
         raise RuntimeError(f"{name} must be contiguous")
+
+
+def _check_gpu(x, name):
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+
+
+def _check_rows(x, name):
+    """A GPU tensor whose last dimension is dense and whose rows begin at multiples of 16 bytes; the other
+    strides are free (a transposed or sliced view is fine).  Returns the strides of the other dimensions,
+    in elements (0 for a dimension of one element, whose stride means nothing)."""
+    _check_gpu(x, name)
+    if x.numel() == 0:
+        return [0] * (x.dim() - 1)
+    strides = [s if n > 1 else 0 for s, n in zip(x.stride()[:-1], x.shape[:-1])]
+    size = x.element_size()
+    if (x.stride(-1) != 1 and x.shape[-1] != 1) or x.data_ptr() % 16 or any(s * size % 16 for s in strides):
+        raise RuntimeError(f"{name} must have a dense last dimension and rows that begin at multiples of 16 bytes")
+    return strides
+
+
+def _check_ints(x, shape, ref, name):
+    _check_input(x, name)
+    _same_device(x, ref, name)
+    if x.dtype != torch.int32 or tuple(x.shape) != tuple(shape):
+        raise RuntimeError(f"{name} must be an int32 tensor of shape {tuple(shape)}, got {x.dtype} {tuple(x.shape)}")
 
 
 def _same_device(x, ref, name):
@@ -454,3 +489,7 @@ def my_matmul_out(out, A, B):
     # `out` is written while A and B are being read: an output that shares storage with an input
     # is refused (the C entry point checks the address ranges and its message surfaces here)
     return _matmul_into(out, A, B)
+
+
+from .window import window_attn_bwd, window_attn_func, window_attn_fwd  # noqa: E402
+from .paged import paged_attn_decode, paged_kv_append, paged_kv_evict  # noqa: E402

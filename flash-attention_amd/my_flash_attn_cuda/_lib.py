@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmyfa_gfx950.so")
 TUNING_LIB_PATH = os.path.join(_HERE, "libmyfa_gfx950_tuning.so")
 
-ABI_VERSION = 3
+ABI_VERSION = 4
 MYFA_F32, MYFA_F16, MYFA_BF16 = 0, 1, 2
 
 # every symbol include/myfa.h declares
@@ -36,6 +36,13 @@ EXPORTS = (
     "myfa_attn_bwd_bhnd",
     "myfa_attn_bwd_bhnd_static_ws",
     "myfa_matmul_f32",
+    "myfa_window_attn_fwd",
+    "myfa_window_attn_bwd_ws_bytes",
+    "myfa_window_attn_bwd",
+    "myfa_paged_append",
+    "myfa_paged_attn_decode_ws_bytes",
+    "myfa_paged_attn_decode",
+    "myfa_paged_evict",
 )
 
 
@@ -83,6 +90,20 @@ def _load():
     lib.myfa_attn_bwd_bhnd_static_ws.restype = ci
     lib.myfa_matmul_f32.argtypes = [vp, vp, vp, i64, i64, i64, vp]
     lib.myfa_matmul_f32.restype = ci
+    lib.myfa_window_attn_fwd.argtypes = [vp] * 6 + [i64] * 6 + [vp] * 3 + [i64, i64, f32, ci, vp]
+    lib.myfa_window_attn_fwd.restype = ci
+    lib.myfa_window_attn_bwd_ws_bytes.argtypes = [i64] * 8
+    lib.myfa_window_attn_bwd_ws_bytes.restype = i64
+    lib.myfa_window_attn_bwd.argtypes = [vp] * 10 + [i64] * 6 + [vp] * 3 + [i64, i64, f32, ci, vp, i64, vp]
+    lib.myfa_window_attn_bwd.restype = ci
+    lib.myfa_paged_append.argtypes = [vp] * 7 + [i64] * 7 + [vp] * 4 + [ci, vp]
+    lib.myfa_paged_append.restype = ci
+    lib.myfa_paged_attn_decode_ws_bytes.argtypes = [i64] * 8 + [ci]
+    lib.myfa_paged_attn_decode_ws_bytes.restype = i64
+    lib.myfa_paged_attn_decode.argtypes = [vp] * 8 + [i64] * 7 + [vp] * 3 + [i64, i64, f32, ci, vp, i64, vp]
+    lib.myfa_paged_attn_decode.restype = ci
+    lib.myfa_paged_evict.argtypes = [vp] * 9 + [i64] * 7 + [vp] * 2 + [i64, i64, i64, ci, vp]
+    lib.myfa_paged_evict.restype = ci
     got = lib.myfa_abi_version()
     if got != ABI_VERSION:
         raise ImportError(f"{LIB_PATH}: ABI version {got}, this package expects {ABI_VERSION}; rebuild")

@@ -34,8 +34,9 @@ extern "C" {
 
 /* 2: the entry points with a caller workspace or the library's own (…_ws, …_static_ws), the fused
  * softmax prologue (…_nd_ex) and 16-bit head dims up to 256 were added; nothing of version 1 changed.
- * 3: myfa_attn_fwd_bhnd_kernel added; nothing of version 2 changed. */
-#define MYFA_ABI_VERSION 3
+ * 3: myfa_attn_fwd_bhnd_kernel added; nothing of version 2 changed.
+ * 4: window attention (myfa_window_attn_*) and the paged cache (myfa_paged_*) added; nothing of version 3 changed. */
+#define MYFA_ABI_VERSION 4
 
 enum {
     MYFA_OK = 0,
@@ -273,6 +274,109 @@ int myfa_attn_bwd_bhnd_static_ws(const void* q, const void* k, const void* v, co
  * csrc/api.cpp:13-38).  Overlapping ranges are refused with MYFA_E_INVALID.
  */
 int myfa_matmul_f32(const float* a, const float* b, float* c, int64_t m, int64_t k, int64_t n, void* stream);
+
+/*
+ * Attention in which a query sees the last `window` keys up to its own position and the first `sinks` keys
+ * of its sequence:
+ *     o[b,h,i] = sum_j p_j v[b,h/G,j],   p = softmax(scale * q[b,h,i] . k[b,h/G,j]) over what is seen,
+ * query i standing at position p = i + Nk - Nq and seeing key j when
+ *     j <= p,  p < len[b],  and  p - j < window or j < sinks.
+ *   q           [B, H, Nq, d], Nq <= Nk;  k, v [B, Hkv, Nk, d], H a multiple of Hkv (G = H / Hkv)
+ *   o, lse      dense [B, H, Nq, d] and float32 [B, H, Nq]; lse (NULL: not wanted) is the natural logarithm of
+ *               the row's sum.  A row that sees nothing (p >= len[b]) is 0 with lse = -infinity.
+ *   seq_lens    int32 [B] on the device, or NULL: every sequence has Nk keys.  Values are clamped to [0, Nk].
+ *   strides     host arrays {batch, head, row} in elements for q, k and v; the last dimension is dense.  All
+ *               strides are multiples of 16 bytes (as are the tensors' addresses), row strides not negative
+ *               and below 2^24 bytes.
+ *   window      >= 1 (more than Nk means Nk);  sinks >= 0;  scale > 0
+ * Element types: MYFA_F16 and MYFA_BF16 with d a multiple of 8 up to 256, MYFA_F32 with d a multiple of 4 up to
+ * 128; otherwise MYFA_E_UNSUPPORTED.  Statistics and sums are float32; P is rounded to the element type.
+ * Keys and values that no row of 128 neighbouring queries sees, and what stands behind a sequence's length,
+ * are not read into the products, whatever their bits are.
+ * No counterpart in the reference, whose attention is unmasked (csrc/api.cpp:168-192).
+ */
+int myfa_window_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* seq_lens,
+                         int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nk, int64_t d,
+                         const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                         int64_t window, int64_t sinks, float scale, int dtype, void* stream);
+
+/*
+ * Gradients of myfa_window_attn_fwd.  o, lse: the forward's results; dout, dq: dense [B, H, Nq, d]; dk, dv: dense
+ * [B, Hkv, Nk, d], summed over the query heads that share them; gradients of rows and keys that nothing sees or
+ * that see nothing are 0.  `workspace`: myfa_window_attn_bwd_ws_bytes(...) bytes, 16-byte aligned, whose contents
+ * before and after mean nothing; it must stay untouched until the call's work on `stream` has finished, and
+ * calls that may overlap need one each.  No atomics: the result depends on the inputs alone.
+ */
+int64_t myfa_window_attn_bwd_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nk, int64_t d,
+                                      int64_t window, int64_t sinks);
+int myfa_window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
+                         void* dq, void* dk, void* dv, const int32_t* seq_lens,
+                         int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nk, int64_t d,
+                         const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+                         int64_t window, int64_t sinks, float scale, int dtype,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * A paged key/value cache: pools k_cache and v_cache of `num_pages` pages [num_pages, Hkv, page, d], each with
+ * strides {page, head, slot} in elements (host array; the last dimension dense, all multiples of 16 bytes).  Key j
+ * of sequence b stands in page block_table[b][j / page], slot j % page; block_table is int32 [B, table_width] on the
+ * device.  Sequences hold at most capacity = table_width * page keys (< 2^31).  Entries behind a sequence's last
+ * page are not read.  A page number outside [0, num_pages) is never turned into an address.
+ * Element types as in myfa_window_attn_fwd.
+ */
+
+/*
+ * Appends n new tokens per sequence: k, v [B, Hkv, n, d] (strides as above, any multiples of 16 bytes) go to the places
+ * seq_lens[b] .. seq_lens[b] + n - 1, or only the first counts[b] of them where counts is not NULL.  seq_lens and
+ * counts are int32 [B] on the device.  Tokens whose place is before 0, behind the capacity, or on a page number
+ * outside the pool are dropped; nothing else is written.  No two tokens of a call may have the same place.
+ */
+int myfa_paged_append(const void* k, const void* v, void* k_cache, void* v_cache, const int32_t* block_table,
+                      const int32_t* seq_lens, const int32_t* counts,
+                      int64_t B, int64_t Hkv, int64_t n, int64_t d, int64_t num_pages, int64_t page, int64_t table_width,
+                      const int64_t* k_strides, const int64_t* v_strides,
+                      const int64_t* kc_strides, const int64_t* vc_strides, int dtype, void* stream);
+
+/*
+ * Attention of one new token per sequence over the cache (the token's own key and value are already there, at
+ * place seq_lens[b] - 1):
+ *     o[b,h] = softmax(scale * q[b,h] . K[b,h/G,j]) V[b,h/G,j]  over j < seq_lens[b] with
+ *              seq_lens[b] - 1 - j < window or j < sinks.            window <= 0: no window, every key is seen.
+ *   q           [B, H, d], strides {batch, head}; o dense [B, H, d]; lse float32 [B, H] or NULL
+ *   weight_sum  float32 [B, Hkv, capacity] or NULL: to the entry of every key that is seen the key's weights,
+ *               summed over the G query heads that share it, are added
+ * A sequence of length 0 (or less) gives 0, lse = -infinity, and leaves its sums alone.  A length beyond the capacity, or
+ * a key that is seen on a page number outside the pool, makes the results of that sequence NaN.
+ * `workspace`: myfa_paged_attn_decode_ws_bytes(...) bytes (may be 0), 16-byte aligned, one per call that may overlap.
+ */
+int64_t myfa_paged_attn_decode_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t d, int64_t page, int64_t table_width,
+                                        int64_t window, int64_t sinks, int with_weights);
+int myfa_paged_attn_decode(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                           const int32_t* seq_lens, void* o, float* lse, float* weight_sum,
+                           int64_t B, int64_t H, int64_t Hkv, int64_t d, int64_t num_pages, int64_t page, int64_t table_width,
+                           const int64_t* q_strides, const int64_t* kc_strides, const int64_t* vc_strides,
+                           int64_t window, int64_t sinks, float scale, int dtype,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Eviction by accumulated attention weight.  Every head of a sequence longer than `budget` keeps its first `sinks`
+ * keys, its last `recent` keys and, of those between, the budget - sinks - recent with the largest weight_sum (equal
+ * sums: the lowest index; NaN above everything).  The kept keys, values and sums are copied, in their order, to the
+ * places 0, 1, ... of new_block_table (int32 [B, new_width], new_width * page >= budget); a sequence within the budget is
+ * copied whole.  The pages of new_block_table must not be among those that the call reads, and none may be there twice.
+ *   weight_sum      float32 [B, Hkv, table_width * page], read only
+ *   new_weight_sum  float32 [B, Hkv, new_width * page]: the kept sums, 0 behind them
+ *   new_lens        int32 [B]: min(seq_lens[b], budget)
+ *   kept            int32 [B, Hkv, budget]: the kept keys' old places, ascending, -1 behind them
+ * 0 <= sinks, 0 <= recent, sinks + recent <= budget, budget >= 1.  Lengths are clamped to [0, capacity].  A kept key on
+ * an old page number outside the pool is copied as NaN; one whose new page number is outside it is dropped.
+ */
+int myfa_paged_evict(void* k_cache, void* v_cache, const float* weight_sum, const int32_t* block_table,
+                     const int32_t* seq_lens, const int32_t* new_block_table,
+                     float* new_weight_sum, int32_t* new_lens, int32_t* kept,
+                     int64_t B, int64_t Hkv, int64_t d, int64_t num_pages, int64_t page, int64_t table_width, int64_t new_width,
+                     const int64_t* kc_strides, const int64_t* vc_strides,
+                     int64_t budget, int64_t sinks, int64_t recent, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,267 @@
+"""Window attention with sinks, forward and backward, on the GPU against its definition in float64 (window_reference.py
+derives the bounds)."""
+import pytest
+import torch
+
+import window_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module")
+def mfa():
+    import my_flash_attn_cuda
+    assert torch.cuda.is_available()
+    return my_flash_attn_cuda
+
+
+def _inputs(B, H, G, nq, nk, d, dtype, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    make = lambda *s: torch.randn(*s, generator=gen).to(dtype)  # noqa: E731
+    return make(B, H, nq, d), make(B, G, nk, d), make(B, G, nk, d), make(B, H, nq, d)
+
+
+def _visible(B, nq, nk, window, sinks, lens):
+    return torch.stack([ref.seen(nq, nk, window, sinks, nk if lens is None else min(max(lens[b], 0), nk)) for b in range(B)])
+
+
+def _run(mfa, q, k, v, dout, window, sinks, scale, lens):
+    L = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out, lse = mfa.window_attn_fwd(q, k, v, window, sinks=sinks, scale=scale, return_lse=True, seq_lens=L)
+    dq, dk, dv = mfa.window_attn_bwd(dout, q, k, v, out, lse, window, sinks=sinks, scale=scale, seq_lens=L)
+    return {"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv}
+
+
+def _compare(mfa, B, H, G, nq, nk, d, window, sinks, lens, dtype, seed=0):
+    q, k, v, dout = _inputs(B, H, G, nq, nk, d, dtype, seed)
+    scale = d ** -0.5
+    want = ref.attention(q, k, v, _visible(B, nq, nk, window, sinks, lens), scale, dtype, dout)
+    got = _run(mfa, *(t.cuda() for t in (q, k, v, dout)), window, sinks, scale, lens)
+    for name in got:
+        ref.check(name, got[name], want[name])
+
+
+CASES = [
+    # B, H, G, nq, nk, d, window, sinks, lens
+    (1, 1, 1, 1, 1, 64, 1, 0, None),                   # one token
+    (1, 2, 1, 1, 300, 64, 40, 3, None),                # one query at the end of a piece
+    (2, 2, 2, 130, 130, 128, 1, 0, None),              # every query sees itself alone
+    (1, 2, 2, 200, 200, 64, 1000, 0, None),            # window wider than the sequence: causal
+    (1, 4, 2, 333, 333, 128, 64, 4, None),
+    (1, 3, 1, 129, 515, 64, 100, 70, None),            # sinks over more than one tile
+    (1, 2, 1, 300, 300, 64, 17, 300, None),            # everything is a sink
+    (2, 6, 2, 77, 150, 80, 33, 1, [150, 90]),
+    (3, 2, 2, 65, 65, 64, 20, 2, [65, 0, 1]),          # an empty sequence and one of one token
+    (2, 2, 1, 40, 200, 64, 50, 4, [100, 170]),         # a piece that lies behind a sequence's length altogether
+    (1, 8, 1, 257, 257, 128, 90, 5, None),             # eight heads share one
+    (1, 2, 1, 640, 640, 64, 100, 130, None),           # two key blocks hold sinks
+    (1, 1, 1, 150, 150, 16, 30, 2, None),
+    (1, 2, 1, 100, 140, 20, 30, 2, [120]),             # head dims off the 16-byte grid are padded
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+def test_against_definition(mfa, case, dtype):
+    _compare(mfa, *case, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [136, 192, 256])
+def test_wide_heads(mfa, d, dtype):
+    _compare(mfa, 1, 2, 1, 150, 210, d, 60, 3, [200], dtype)
+
+
+def test_long_sequence(mfa):
+    _compare(mfa, 1, 2, 1, 2100, 2100, 128, 300, 4, None, BF16)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gradients_against_differences(mfa, dtype):
+    """The gradients of the definition itself, against central differences of it: what the bounds are held to is the
+    derivative of the forward."""
+    q, k, v, dout = (t.double() for t in _inputs(1, 2, 1, 9, 14, 8, F32, 3))
+    vis = _visible(1, 9, 14, 4, 2, [13])
+    want = ref.attention(q, k, v, vis, 0.4, dtype, dout)
+    for name, t in (("dq", q), ("dk", k), ("dv", v)):
+        for at in [(0, 0, 2, 1), (0, 0, 7, 5), (0, 0, 5, 0)]:
+            h = 1e-5
+            vals = []
+            for sign in (1, -1):
+                x = {"dq": q, "dk": k, "dv": v}[name].clone()
+                x[at] += sign * h
+                args = [x if n == name else y for n, y in (("dq", q), ("dk", k), ("dv", v))]
+                vals.append(float((ref.attention(*args, vis, 0.4, dtype)["out"][0] * dout).sum()))
+            assert abs((vals[0] - vals[1]) / (2 * h) - float(want[name][0][at])) < 1e-7
+    got = _run(mfa, *(t.to(dtype).cuda() for t in (q, k, v, dout)), 4, 2, 0.4, [13])
+    rounded = ref.attention(*(t.to(dtype) for t in (q, k, v)), vis, 0.4, dtype, dout.to(dtype))
+    for name in got:
+        ref.check(name, got[name], rounded[name])
+
+
+@pytest.mark.parametrize("fill", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_padding_may_hold_anything(mfa, fill, dtype):
+    lens = [100, 37, 0]
+    q, k, v, dout = _inputs(3, 4, 2, 100, 100, 64, dtype, 1)
+    want = ref.attention(q, k, v, _visible(3, 100, 100, 30, 2, lens), 0.125, dtype, dout)
+    for b, n in enumerate(lens):
+        for t in (q, k, v, dout):
+            t[b, :, n:] = fill
+    got = _run(mfa, *(t.cuda() for t in (q, k, v, dout)), 30, 2, 0.125, lens)
+    for name in got:
+        ref.check(name, got[name], want[name])
+
+
+def test_keys_before_every_window_may_hold_anything(mfa):
+    q, k, v, dout = _inputs(1, 2, 1, 50, 400, 64, BF16, 2)
+    vis = _visible(1, 50, 400, 30, 2, None)
+    want = ref.attention(q, k, v, vis, 0.125, BF16, dout)
+    hidden = ~vis.any(1)[0]
+    k[:, :, hidden], v[:, :, hidden] = float("nan"), float("inf")
+    got = _run(mfa, *(t.cuda() for t in (q, k, v, dout)), 30, 2, 0.125, None)
+    for name in got:
+        ref.check(name, got[name], want[name])
+
+
+def test_strided_views(mfa):
+    """(B, N, H, d) layouts and slices of one fused projection give what dense copies give, bit for bit."""
+    torch.manual_seed(0)
+    fused = torch.randn(2, 190, 8, 64, device="cuda", dtype=BF16)
+    q, k, v = fused[:, :, :4].transpose(1, 2), fused[:, :, 4:6].transpose(1, 2), fused[:, :, 6:].transpose(1, 2)
+    dout = torch.randn(2, 4, 190, 64, device="cuda", dtype=BF16)
+    lens = [190, 111]
+    a = _run(mfa, q, k, v, dout, 50, 4, 0.125, lens)
+    b = _run(mfa, q.contiguous(), k.contiguous(), v.contiguous(), dout, 50, 4, 0.125, lens)
+    for name in a:
+        assert torch.equal(a[name], b[name]), name
+    one = k[:, :, :1].expand(2, 2, 190, 64)              # rows of stride 0
+    a = _run(mfa, q, one, v, dout, 50, 4, 0.125, lens)
+    b = _run(mfa, q, one.contiguous(), v, dout, 50, 4, 0.125, lens)
+    for name in a:
+        assert torch.equal(a[name], b[name]), name
+
+
+def test_same_result_every_time(mfa):
+    q, k, v, dout = (t.cuda() for t in _inputs(2, 8, 2, 700, 700, 128, BF16, 4))
+    first = _run(mfa, q, k, v, dout, 128, 4, 0.1, [700, 600])
+    for _ in range(3):
+        again = _run(mfa, q, k, v, dout, 128, 4, 0.1, [700, 600])
+        for name in first:
+            assert torch.equal(first[name], again[name]), name
+
+
+def test_large_logits(mfa):
+    """Logits of some thousands: the running maximum moves far, and weights underflow."""
+    q, k, v, dout = _inputs(1, 1, 1, 200, 200, 64, F32, 5)
+    want = ref.attention(q * 30, k * 30, v, _visible(1, 200, 200, 90, 1, None), 1.0, F32)
+    out, lse = mfa.window_attn_fwd((q * 30).cuda(), (k * 30).cuda(), v.cuda(), 90, sinks=1, scale=1.0, return_lse=True)
+    ref.check("out", out, want["out"])
+    ref.check("lse", lse, want["lse"])
+
+
+def test_causal_case_agrees_with_flash_attn(mfa):
+    q, k, v, _ = (t.cuda() for t in _inputs(2, 2, 2, 257, 257, 128, BF16, 6))
+    want = ref.attention(*(t.cpu() for t in (q, k, v)), _visible(2, 257, 257, 257, 0, None), 0.09, BF16)
+    ref.check("flash", mfa.flash_attn_fwd(q, k, v, scale=0.09, return_lse=True, causal=True)[0], want["out"])
+    ref.check("window", mfa.window_attn_fwd(q, k, v, 257, scale=0.09), want["out"])
+
+
+def test_autograd(mfa):
+    q, k, v, dout = (t.cuda() for t in _inputs(2, 4, 2, 90, 90, 64, BF16, 7))
+    lens = torch.tensor([90, 50], dtype=torch.int32, device="cuda")
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = mfa.window_attn_func(*leaves, 20, sinks=2, scale=0.125, seq_lens=lens)
+    grads = torch.autograd.grad(out, leaves, dout.transpose(1, 2).contiguous().transpose(1, 2))     # a strided gradient
+    want = _run(mfa, q, k, v, dout, 20, 2, 0.125, [90, 50])
+    for name, g in zip(("dq", "dk", "dv"), grads):
+        assert torch.equal(g, want[name]), name
+
+
+def test_other_stream(mfa):
+    q, k, v, dout = (t.cuda() for t in _inputs(1, 4, 2, 500, 500, 128, BF16, 8))
+    want = _run(mfa, q, k, v, dout, 100, 4, 0.1, None)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = _run(mfa, q, k, v, dout, 100, 4, 0.1, None)
+    side.synchronize()
+    for name in got:
+        assert torch.equal(got[name], want[name]), name
+
+
+def test_graph_replays(mfa):
+    """Forward and backward captured, replayed over new inputs with eager work in between."""
+    L = torch.tensor([300, 200], dtype=torch.int32, device="cuda")
+    static = [t.cuda() for t in _inputs(2, 4, 2, 300, 300, 64, BF16, 9)]
+
+    def step():
+        out, lse = mfa.window_attn_fwd(*static[:3], 40, sinks=4, scale=0.125, return_lse=True, seq_lens=L)
+        return (out, lse, *mfa.window_attn_bwd(static[3], *static[:3], out, lse, 40, sinks=4, scale=0.125, seq_lens=L))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in range(4):
+        for t, x in zip(static, _inputs(2, 4, 2, 300, 300, 64, BF16, 20 + seed)):
+            t.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
+
+
+def test_refusals(mfa):
+    q, k, v, dout = (t.cuda() for t in _inputs(1, 4, 2, 32, 48, 64, BF16, 0))
+    lens = torch.tensor([48], dtype=torch.int32, device="cuda")
+    bad = [
+        (dict(window=0), "window"), (dict(window=8, sinks=-1), "sinks"), (dict(window=8, scale=0.0), "scale"),
+        (dict(window=8, scale=float("nan")), "scale"), (dict(window=8, seq_lens=lens.long()), "int32"),
+        (dict(window=8, seq_lens=torch.tensor([48, 48], dtype=torch.int32, device="cuda")), "int32"),
+        (dict(window=8, seq_lens=lens.cpu()), "CUDA tensor"),
+    ]
+    for kw, match in bad:
+        with pytest.raises(RuntimeError, match=match):
+            mfa.window_attn_fwd(q, k, v, **kw)
+    with pytest.raises(RuntimeError, match="Wrong sizes"):
+        mfa.window_attn_fwd(k, q[:, :2], q[:, :2], 8)                  # more queries than keys
+    with pytest.raises(RuntimeError, match="Wrong sizes"):
+        mfa.window_attn_fwd(q, k, v[:, :, 1:], 8)
+    with pytest.raises(RuntimeError, match="multiple"):
+        mfa.window_attn_fwd(q[:, :3], k, v, 8)
+    with pytest.raises(RuntimeError, match="Scalar type"):
+        mfa.window_attn_fwd(q, k.half(), v, 8)
+    with pytest.raises(RuntimeError, match="unsupported dtype"):
+        mfa.window_attn_fwd(q.double(), k.double(), v.double(), 8)
+    with pytest.raises(RuntimeError, match="head dims up to"):
+        mfa.window_attn_fwd(*(torch.zeros(1, 2, 8, 264, device="cuda", dtype=BF16) for _ in range(3)), 8)
+    with pytest.raises(RuntimeError, match="head dims up to"):
+        mfa.window_attn_fwd(*(torch.zeros(1, 2, 8, 136, device="cuda") for _ in range(3)), 8)
+    wide = torch.zeros(1, 4, 32, 65, device="cuda", dtype=BF16)
+    with pytest.raises(RuntimeError, match="16 bytes"):
+        mfa.window_attn_fwd(wide[..., :64], k, v, 8)
+    with pytest.raises(RuntimeError, match="16 bytes"):
+        mfa.window_attn_fwd(q.transpose(2, 3).contiguous().transpose(2, 3), k, v, 8)
+    out, lse = mfa.window_attn_fwd(q, k, v, 8, return_lse=True)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        mfa.window_attn_bwd(dout.transpose(1, 2).contiguous().transpose(1, 2), q, k, v, out, lse, 8)
+    with pytest.raises(RuntimeError, match="lse must"):
+        mfa.window_attn_bwd(dout, q, k, v, out, lse[:, :, :-1].contiguous(), 8)
+    with pytest.raises(RuntimeError, match="Wrong sizes"):
+        mfa.window_attn_bwd(dout[:, :2].contiguous(), q, k, v, out, lse, 8)
+
+
+def test_empty_sizes(mfa):
+    q, k, v = (torch.empty(*s, device="cuda", dtype=BF16) for s in ((0, 2, 5, 64), (0, 2, 5, 64), (0, 2, 5, 64)))
+    assert mfa.window_attn_fwd(q, k, v, 4).shape == (0, 2, 5, 64)
+    q, k = torch.empty(1, 2, 0, 64, device="cuda", dtype=BF16), torch.ones(1, 2, 7, 64, device="cuda", dtype=BF16)
+    out, lse = mfa.window_attn_fwd(q, k, k, 4, return_lse=True)
+    assert out.shape == (1, 2, 0, 64)
+    dq, dk, dv = mfa.window_attn_bwd(out, q, k, k, out, lse, 4, sinks=1)
+    assert dq.numel() == 0 and not dk.any() and not dv.any()
