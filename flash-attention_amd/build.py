@@ -2,10 +2,12 @@
 """Builds libmyfa_gfx950.so: hipcc, gfx950 only, in-tree.
 
 Takes the place of the reference's setup.py CUDAExtension build
-(setup.py:107-143 of the reference: nvcc, sm_75, ninja).  There is no
-torch C++ extension here -- the library is a plain C-ABI shared object that the
-Python host layer loads with ctypes -- so the build is one hipcc invocation per
-translation unit and a link.  Objects are cached under csrc/.obj keyed on the
+(setup.py:107-143 of the reference: nvcc, sm_75, ninja).  The
+kernels are a plain C-ABI shared object that the Python host layer loads with
+ctypes, so the build is one hipcc invocation per
+translation unit and a link.  Beside it goes one Python extension module without
+device code, _host.so (csrc/host_binding.cpp, g++ against torch's headers): the host
+layer of the operators whose calls take microseconds.  Objects are cached under csrc/.obj keyed on the
 source and header mtimes.
 """
 import os
@@ -25,6 +27,9 @@ LIB = os.path.join(PKG, "libmyfa_gfx950.so")
 # exported functions (csrc/tuning.h).  For tools/ and the tests that compare kernel variants;
 # the package never loads it.
 LIB_TUNING = os.path.join(PKG, "libmyfa_gfx950_tuning.so")
+
+HOST_SOURCE = "host_binding.cpp"
+HOST_LIB = os.path.join(PKG, "_host.so")
 
 SOURCES = ["c_abi.hip", "softmax_rows.hip", "softmax_strided.hip", "attn_fwd_f32.hip", "attn_fwd_dispatch.hip", "attn_fwd_mfma.hip",
            "attn_fwd_mfma16.hip", "attn_fwd_stream.hip", "attn_fwd_mfma256.hip", "attn_bwd_mfma.hip", "attn_bwd_wide.hip", "attn_bwd_f32.hip", "matmul_f32.hip",
@@ -87,10 +92,35 @@ def _build_one(lib, objdir, flags, force, verbose):
     return lib
 
 
+def build_host(force=False, verbose=True):
+    """The host extension module, linked against the shipped library beside it and torch."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    src, tag = os.path.join(CSRC, HOST_SOURCE), os.path.join(OBJ, "_host.cmd")
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-unknown-pragmas", "-DUSE_ROCM", "-D__HIP_PLATFORM_AMD__=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + INCLUDE,
+           *("-isystem" + d for d in (*cpp_extension.include_paths(), "/opt/rocm/include", sysconfig.get_paths()["include"])),
+           src, "-o", HOST_LIB, "-L" + PKG, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN",
+           *("-L" + d for d in cpp_extension.library_paths()), "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_python"]
+    text = " ".join(cmd) + " torch " + torch.__version__
+    stamp = max(os.path.getmtime(src), os.path.getmtime(os.path.join(INCLUDE, "myfa.h")), os.path.getmtime(__file__))
+    if force or not os.path.exists(HOST_LIB) or os.path.getmtime(HOST_LIB) < stamp or not os.path.exists(tag) or open(tag).read() != text:
+        subprocess.check_call(cmd)
+        with open(tag, "w") as f:
+            f.write(text)
+        if verbose:
+            print(f"[myfa] linked {HOST_LIB}")
+    elif verbose:
+        print(f"[myfa] up to date: {HOST_LIB}")
+
+
 def build_library(force=False, verbose=True, extra_flags=(), tuning=True):
     """Compile every HIP source for gfx950 and link the shared library (and, unless tuning=False,
     its tuning flavour)."""
     lib = _build_one(LIB, OBJ, list(extra_flags), force, verbose)
+    build_host(force, verbose)
     if tuning:
         _build_one(LIB_TUNING, OBJ + "_tuning", [*extra_flags, "-DMYFA_TUNING"], force, verbose)
     return lib

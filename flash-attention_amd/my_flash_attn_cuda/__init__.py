@@ -48,34 +48,6 @@ def _check_input(x, name):
         raise RuntimeError(f"{name} must be contiguous")
 
 
-def _check_gpu(x, name):
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if not x.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA tensor")
-
-
-def _check_rows(x, name):
-    """A GPU tensor whose last dimension is dense and whose rows begin at multiples of 16 bytes; the other
-    strides are free (a transposed or sliced view is fine).  Returns the strides of the other dimensions,
-    in elements (0 for a dimension of one element, whose stride means nothing)."""
-    _check_gpu(x, name)
-    if x.numel() == 0:
-        return [0] * (x.dim() - 1)
-    strides = [s if n > 1 else 0 for s, n in zip(x.stride()[:-1], x.shape[:-1])]
-    size = x.element_size()
-    if (x.stride(-1) != 1 and x.shape[-1] != 1) or x.data_ptr() % 16 or any(s * size % 16 for s in strides):
-        raise RuntimeError(f"{name} must have a dense last dimension and rows that begin at multiples of 16 bytes")
-    return strides
-
-
-def _check_ints(x, shape, ref, name):
-    _check_input(x, name)
-    _same_device(x, ref, name)
-    if x.dtype != torch.int32 or tuple(x.shape) != tuple(shape):
-        raise RuntimeError(f"{name} must be an int32 tensor of shape {tuple(shape)}, got {x.dtype} {tuple(x.shape)}")
-
-
 def _same_device(x, ref, name):
     if x.device != ref.device:
         raise RuntimeError(f"{name} is on {x.device}, expected {ref.device}: all operands must be on one device")

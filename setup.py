@@ -2,10 +2,9 @@
 """Installs the MI355X drop-in for the reference's `my_flash_attn_cuda` extension.
 
 Takes the place of the reference's setup.py (CUDAExtension "my_flash_attn_cuda", nvcc,
-sm_75; setup.py:107-143 there).  Nothing here goes through torch.utils.cpp_extension:
-the kernels are compiled by hipcc for gfx950 into one C-ABI shared library
-(flash-attention_amd/build.py) that ships inside the pure-Python package of the same
-import name.  No git submodules are fetched and no compiler is forced.
+sm_75; setup.py:107-143 there).  The kernels are compiled by hipcc for gfx950 into one
+C-ABI shared library (flash-attention_amd/build.py) that ships inside the Python package
+of the same import name, beside one small host extension module.  No git submodules are fetched and no compiler is forced.
 
     python setup.py build_ext --inplace     # just build libmyfa_gfx950.so in-tree
     pip install -e .                        # development install
@@ -54,7 +53,7 @@ setup(
                 "drop-in for my_flash_attn_cuda",
     package_dir={"": "flash-attention_amd"},
     packages=["my_flash_attn_cuda"],
-    package_data={"my_flash_attn_cuda": ["libmyfa_gfx950.so"]},
+    package_data={"my_flash_attn_cuda": ["libmyfa_gfx950.so", "_host.so"]},
     python_requires=">=3.9",
     cmdclass={"build_ext": BuildHip, "build_py": BuildPyWithHip},
 )
