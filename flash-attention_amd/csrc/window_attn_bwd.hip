@@ -20,6 +20,7 @@
 // its keys fill the registers) and forms S and dP for each half again.
 // P and dS are rounded to the element type as operands; everything else is float32.  Rows and keys that
 // have no visible partner in the workgroup are fetched as zeros, so whatever stands there stays out.
+#include "attn_bwd_plan.h"
 #include "window_attn_common.h"
 
 namespace myfa {
@@ -179,6 +180,185 @@ window_bwd_dq_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T
     }
 }
 
+// dQ for 16-bit elements and up to 128 columns.  The tile's 64 keys are two blocks of 32, staggered so that
+// the vector part of one block runs in the shadow of the other's matrix products:
+//     S0, dP0 | S1, dP1 with dS0 | barrier | dQ += block 0 with dS1 | dQ += block 1
+// K in a ring of three, V in one of two: behind the tile's last transposing read (which waits for every
+// LDS-DMA load in flight) K(t + 2) and V(t + 2) are requested; the barrier of tile t + 1 finds them complete.
+// Two workgroups a CU (160 KiB of LDS between them).
+template <typename T, int D>
+__global__ void __launch_bounds__(256, 2)
+window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
+                       const T* __restrict__ dOg, const float* __restrict__ st, T* __restrict__ dQg,
+                       WindowShape w, int nqp, int64_t rows, int nqblk, int nwg) {
+    using M = Mma<T>;
+    using R = TileReader<T, D>;
+    constexpr int BN = 64, KS = R::KS, DB = R::DB, TILE_B = BN * R::RB, FW = 4;
+    __shared__ __attribute__((aligned(1024))) char lds[5 * TILE_B];   // K0 K1 K2 V0 V1
+
+    const int lid = xcd_range_id(blockIdx.x, nwg);
+    const int bh = lid / nqblk;
+    const int b = bh / w.H, head = bh - b * w.H, kvh = head / (w.H / w.Hkv);
+    const int q0 = (lid - bh * nqblk) * 128;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5;
+    const int len = w.lens ? min(max(w.lens[b], 0), w.Nk) : w.Nk;
+    const int shift = w.Nk - w.Nq;
+    const int pa = q0 + shift, pz = min(min(q0 + 128, w.Nq) + shift, len);
+    const int lo = max(0, pa - w.window + 1);
+    const int t_win = lo / BN, t_end = pz > pa ? (pz + BN - 1) / BN : t_win;
+    const int n_sink = pz > pa ? min((min(w.sinks, pz) + BN - 1) / BN, t_win) : 0;
+    const int ntiles = n_sink + (t_end - t_win);
+
+    const int qrow = q0 + 32 * wave + r;
+    const int p_own = qrow + shift;
+    const bool live = qrow < w.Nq && p_own < len;
+    const int p_hi = live ? p_own : -1, p_lo = p_own - w.window + 1;
+    const int wave_lo = q0 + 32 * wave + shift, wave_hi = min(wave_lo + 32, pz) - 1;
+
+    const T* Kh = Kg + b * w.ks[0] + kvh * w.ks[1];
+    const T* Vh = Vg + b * w.vs[0] + kvh * w.vs[1];
+    const R rd(lane);
+    const TileFetch<T, D, BN, 256> kfetch(tid, w.ks[2], w.d), vfetch(tid, w.vs[2], w.d);
+    auto first_key = [&](int t) __attribute__((always_inline)) { return (t < n_sink ? t : t - n_sink + t_win) * BN; };
+    auto fetch = [&](int t, int kslot) __attribute__((always_inline)) {
+        if (t >= ntiles) return;
+        const int k0 = first_key(t);
+        char* kt = lds + kslot * TILE_B;
+        char* vt = lds + (3 + (t & 1)) * TILE_B;
+        if (k0 + BN <= pz && (k0 >= lo || k0 + BN <= w.sinks)) {
+            kfetch.fetch(Kh + (int64_t)k0 * w.ks[2], kt, true, [](int) { return true; });
+            vfetch.fetch(Vh + (int64_t)k0 * w.vs[2], vt, true, [](int) { return true; });
+        } else {
+            auto keep = [&](int row) { const int k = k0 + row; return (k < pz) & ((k >= lo) | (k < w.sinks)); };
+            kfetch.fetch(Kh + (int64_t)k0 * w.ks[2], kt, false, keep);
+            vfetch.fetch(Vh + (int64_t)k0 * w.vs[2], vt, false, keep);
+        }
+    };
+    fetch(0, 0);
+    fetch(1, 1);
+
+    s16x8 qf[KS], of[KS];
+    {
+        const int row = min(qrow, w.Nq - 1);
+        const T* qp = Qg + b * w.qs[0] + head * w.qs[1] + (int64_t)row * w.qs[2];
+        const T* op = dOg + ((int64_t)bh * w.Nq + row) * w.d;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int c = (2 * ks + h) * 8;
+            qf[ks] = s16x8{};
+            of[ks] = s16x8{};
+            if (c < w.d) {
+                qf[ks] = *reinterpret_cast<const s16x8*>(qp + c);
+                of[ks] = *reinterpret_cast<const s16x8*>(op + c);
+            }
+        }
+    }
+    const int64_t srow = (int64_t)bh * nqp + min(qrow, nqp - 1);
+    const float lse2 = st[srow], ndelta = st[rows + srow];
+    const float sl2 = w.scale * kLog2eW;
+
+    f32x16 dq[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dq[db][i] = 0.f;
+    tile_ready();
+
+    int cur = 0, nxt = 1, fre = 2;                 // K slots of tiles t, t + 1, t + 2
+    for (int t = 0; t < ntiles; ++t) {
+        const int k0 = first_key(t);
+        const char* Kb = lds + cur * TILE_B;
+        const char* Vb = lds + (3 + (t & 1)) * TILE_B;
+        const bool some = !(k0 > wave_hi || (k0 + BN <= wave_lo - w.window + 1 && k0 >= w.sinks));
+        const bool edge = !(k0 + BN - 1 <= wave_lo && wave_lo + 31 < len && wave_lo + 31 - shift < w.Nq &&
+                            (k0 >= wave_lo + 31 - w.window + 1 || k0 + BN <= w.sinks));
+        f32x16 s[2], dp[2];
+        typename M::vec8 sb[4];
+        auto pds = [&](int kb, int i) __attribute__((always_inline)) {
+            s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], sl2, -lse2)) * (dp[kb][i] + ndelta);
+        };
+        auto finish = [&](int kb) __attribute__((always_inline)) {
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int key = k0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
+                    if (!((key <= p_hi) & ((key >= p_lo) | (key < w.sinks)))) s[kb][i] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sb[2 * kb + (i >> 3)][i & 7] = (T)s[kb][i];
+        };
+        if (some) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) { s[kb][i] = 0.f; dp[kb][i] = 0.f; }
+            auto block = [&](auto kb_, auto&& after) __attribute__((always_inline)) {
+                constexpr int kb = decltype(kb_)::value;
+                mma_stream<2 * KS, FW>([&](auto ic) __attribute__((always_inline)) {
+                                           constexpr int i = decltype(ic)::value;
+                                           return rd.row(i / KS ? Vb : Kb, kb, i % KS);
+                                       },
+                                       [&](auto ic, s16x8 a) __attribute__((always_inline)) {
+                                           constexpr int i = decltype(ic)::value;
+                                           if constexpr (i / KS) dp[kb] = mma_chunk<T>(a, of[i % KS], dp[kb]);
+                                           else s[kb] = mma_chunk<T>(a, qf[i % KS], s[kb]);
+                                       }, after);
+            };
+            constexpr int EP = 16 / (2 * KS);
+            block(IC<0>{}, [](auto) {});
+            block(IC<1>{}, [&](auto ic) __attribute__((always_inline)) {
+#pragma unroll
+                for (int e = 0; e < EP; ++e) pds(0, EP * decltype(ic)::value + e);
+            });
+            finish(0);
+        }
+        tile_ready();
+        if (some) {
+            auto add = [&](auto kb_, auto&& after) __attribute__((always_inline)) {
+                constexpr int kb = decltype(kb_)::value;
+                mma_stream<2 * DB, FW>([&](auto ic) __attribute__((always_inline)) {
+                                           constexpr int i = decltype(ic)::value;
+                                           return rd.transposed(Kb, kb, i / DB, i % DB);
+                                       },
+                                       [&](auto ic, s16x8 a) __attribute__((always_inline)) {
+                                           constexpr int i = decltype(ic)::value;
+                                           dq[i % DB] = M::run(a, sb[2 * kb + i / DB], dq[i % DB]);
+                                       }, after);
+            };
+            constexpr int EP = 16 / (2 * DB);
+            add(IC<0>{}, [&](auto ic) __attribute__((always_inline)) {
+#pragma unroll
+                for (int e = 0; e < EP; ++e) pds(1, EP * decltype(ic)::value + e);
+            });
+            finish(1);
+            add(IC<1>{}, [&](auto ic) __attribute__((always_inline)) {
+                if constexpr (decltype(ic)::value == (2 * DB > FW ? 2 * DB - FW : 0)) fetch(t + 2, fre);
+            });
+        } else {
+            fetch(t + 2, fre);
+        }
+        const int was = cur;
+        cur = nxt; nxt = fre; fre = was;
+    }
+
+    if (qrow < w.Nq) {
+        T* row = dQg + ((int64_t)bh * w.Nq + qrow) * w.d;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int c = 32 * db + 8 * g + 4 * h;
+                typename M::vec4 x;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = live ? (T)(dq[db][4 * g + j] * w.scale) : (T)0.f;
+                if (c < w.d) *reinterpret_cast<typename M::vec4*>(row + c) = x;
+            }
+    }
+}
+
 // ---------------------------------------------------------------- dK, dV
 template <typename T, int D>
 __global__ void __launch_bounds__(256, D * sizeof(T) <= 128 ? 2 : 1)
@@ -327,6 +507,243 @@ window_bwd_dkv_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const 
         }
 }
 
+// dK, dV for 16-bit elements and up to 128 columns: one wave per SIMD with the keys' fragments and both
+// accumulators in its 512 registers, the tile one pinned stream of 8 KS MFMAs whose shadows take the
+// vector work in the order that attn_bwd_plan.h plans.  S and dP are pinned to vector registers (Mma::acc_v),
+// with the distance to their readers that this asks for; dK and dV to the accumulator registers by use.  Three
+// buffers of Q and dO: tile j + 2 is requested in the last steps of tile j, behind its last transposing read.
+// The tiles of a query head in which every row sees every key of the workgroup carry no mask code.
+template <typename T, int D>
+__global__ void __launch_bounds__(256, 1)
+window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
+                        const T* __restrict__ dOg, const float* __restrict__ st, T* __restrict__ dKg, T* __restrict__ dVg,
+                        float* __restrict__ parts, WindowShape w, int nqp, int64_t rows, int nkblk, int nsb, int ns, int nwg) {
+    using M = Mma<T>;
+    using vec8 = typename M::vec8;
+    using vec4 = typename M::vec4;
+    using R = TileReader<T, D>;
+    constexpr int BQ = 64, KS = R::KS, DB = R::DB, TILE_B = BQ * R::RB;
+    using F = TileFetch<T, D, BQ, 256>;
+    constexpr int LPT = F::LPT;
+    __shared__ __attribute__((aligned(1024))) char lds[6 * TILE_B + 6 * BQ * 4];    // Q0 Q1 Q2 dO0 dO1 dO2, [buf][lse2 | -delta][64]
+    float* stat = reinterpret_cast<float*>(lds + 6 * TILE_B);
+
+    const int units = nsb * ns + (nkblk - nsb);
+    const int lid = xcd_range_id(blockIdx.x, nwg);
+    const int bg = lid / units, unit = lid - bg * units;
+    const bool split = unit < nsb * ns;
+    const int kblk = split ? unit / ns : unit - nsb * ns + nsb, part = split ? unit - kblk * ns : 0, nparts = split ? ns : 1;
+    const int b = bg / w.Hkv, kvh = bg - b * w.Hkv, group = w.H / w.Hkv;
+    const int k0 = kblk * 128;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5;
+    const int len = w.lens ? min(max(w.lens[b], 0), w.Nk) : w.Nk;
+    const int shift = w.Nk - w.Nq;
+    // positions that see some key of the block: [pa, pz); tiles of a head: nt from tq0 on
+    const int pa = max(k0, shift), pz = k0 < w.sinks ? len : min(len, k0 + 127 + w.window);
+    const int tq0 = (pa - shift) / BQ, nt = pz > pa ? (pz - shift + BQ - 1) / BQ - tq0 : 0;
+    const int total = nt * group;
+    const int j0 = (int)((int64_t)total * part / nparts), j1 = (int)((int64_t)total * (part + 1) / nparts);
+    // tiles [m0, m1) of a head are whole: positions at or behind the block's last key, inside the length, and
+    // inside the window of its first key unless all of it are sinks
+    const int whole_end = k0 + 127 >= w.Nk ? 0 : k0 + 128 <= w.sinks ? len : min(len, k0 + w.window);
+    const int m0 = max(k0 + 127 - shift - tq0 * BQ + BQ - 1, 0) / BQ, m1 = max(whole_end - shift - tq0 * BQ, 0) / BQ;
+
+    const int krow = k0 + 32 * wave + r;
+    const int p_lo = krow, p_hi = krow >= w.Nk ? -1 : krow < w.sinks ? len - 1 : min(len - 1, krow + w.window - 1);
+
+    s16x8 kf_[KS], vf_[KS];
+    {
+        const int row = min(krow, w.Nk - 1);
+        const T* kp = Kg + b * w.ks[0] + kvh * w.ks[1] + (int64_t)row * w.ks[2];
+        const T* vp = Vg + b * w.vs[0] + kvh * w.vs[1] + (int64_t)row * w.vs[2];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int c = (2 * ks + h) * 8;
+            kf_[ks] = s16x8{};
+            vf_[ks] = s16x8{};
+            if (c < w.d) {
+                kf_[ks] = *reinterpret_cast<const s16x8*>(kp + c);
+                vf_[ks] = *reinterpret_cast<const s16x8*>(vp + c);
+            }
+        }
+    }
+    vec8 kf[KS], vf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) { kf[ks] = __builtin_bit_cast(vec8, kf_[ks]); vf[ks] = __builtin_bit_cast(vec8, vf_[ks]); }
+    const float sl2 = w.scale * kLog2eW;
+
+    const R rd(lane);
+    const F qfetch(tid, w.qs[2], w.d), ofetch(tid, w.d, w.d);
+    // where tile j (clamped to the last) of the flat list begins
+    struct At { const T *q, *o; const float* s; int p; };
+    auto at = [&](int j) __attribute__((always_inline)) {
+        j = min(j, j1 - 1);
+        const int g = j / nt, i0 = (tq0 + j - g * nt) * BQ, head = kvh * group + g;
+        const int64_t bh = (int64_t)b * w.H + head;
+        return At{Qg + b * w.qs[0] + head * w.qs[1] + (int64_t)i0 * w.qs[2], dOg + (bh * w.Nq + i0) * w.d, st + bh * nqp + i0, i0 + shift};
+    };
+    // piece p of a tile's fetch: even p chunk set p / 2 of Q, odd p that of dO (p < 2 LPT), then the row statistics (wave 0).
+    // Rows that see no key of the block read as zeros.
+    auto fetch_piece = [&](const At& a, int buf, auto p_) __attribute__((always_inline)) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        constexpr int p = decltype(p_)::value;
+        if constexpr (p < 2 * LPT) {
+            const F& f = p % 2 ? ofetch : qfetch;
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(p % 2 ? a.o : a.q), 0, kTileBytesMax, 0x00020000);
+            const int off = (unsigned)(a.p + f.row[p / 2] - pa) < (unsigned)(pz - pa) ? f.off[p / 2] : kOffPast;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(lds + ((p % 2) * 3 + buf) * TILE_B + 1024 * (wave * LPT + p / 2)), 16, off, 0, 0, 0);
+        } else if (wave == 0) {
+            const __amdgpu_buffer_rsrc_t rl = __builtin_amdgcn_make_buffer_rsrc((void*)a.s, 0, BQ * 4, 0x00020000);
+            const __amdgpu_buffer_rsrc_t rdl = __builtin_amdgcn_make_buffer_rsrc((void*)(a.s + rows), 0, BQ * 4, 0x00020000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rl, (lds_void*)(stat + buf * 2 * BQ), 4, lane * 4, 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rdl, (lds_void*)(stat + buf * 2 * BQ + BQ), 4, lane * 4, 0, 0, 0);
+        }
+#endif
+    };
+    auto fetch_tile = [&](int j, int buf) __attribute__((always_inline)) {
+        const At a = at(j);
+        static_for<2 * LPT + 1>([&](auto ic) __attribute__((always_inline)) { fetch_piece(a, buf, ic); });
+    };
+
+    f32x16 dk[DB], dv[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { dk[db][i] = 0.f; dv[db][i] = 0.f; }
+
+    using Plan = DkvPlanFor<KS>;
+    static_assert(Plan::plan.ok && 4 * DB == 2 * KS, "every vector operation placed before its deadline");
+    constexpr int NSTEP = 8 * KS, FW = 8, PSTEP = FW / (2 * LPT);
+    static_assert(PSTEP >= 1 && PSTEP * 2 * LPT == FW, "the tile's loads fill its last FW steps");
+    int cur = 0, nxt = 1, fre = 2;
+
+    auto tile = [&](int j, auto edge_) __attribute__((always_inline)) {
+        constexpr bool EDGE = decltype(edge_)::value != 0;
+        const char* Qb = lds + cur * TILE_B;
+        const char* dOb = lds + (3 + cur) * TILE_B;
+        const float* lse2b = stat + cur * 2 * BQ;
+        const int pt = (tq0 + j % nt) * BQ + shift;
+        const At next = at(j + 2);
+
+        f32x16 s[2], dp[2];
+        f32x4 l4[2][4];
+        vec8 pb[4], sb[4];
+#pragma unroll
+        for (int qb = 0; qb < 2; ++qb)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                l4[qb][g] = *reinterpret_cast<const f32x4*>(lse2b + 32 * qb + 8 * g + 4 * h);
+                const f32x4 nd = *reinterpret_cast<const f32x4*>(lse2b + BQ + 32 * qb + 8 * g + 4 * h);
+                dp[qb][4 * g] = nd[0]; dp[qb][4 * g + 1] = nd[1]; dp[qb][4 * g + 2] = nd[2]; dp[qb][4 * g + 3] = nd[3];
+            }
+        // element c = 32 qb + 8 (i >> 2) + (i & 3) of this lane is masked iff c > c_hi or c < c_lo
+        [[maybe_unused]] const int c_hi = p_hi - (pt + 4 * h), c_lo = p_lo - (pt + 4 * h);
+
+        auto frag = [&](auto gc) __attribute__((always_inline)) -> s16x8 {
+            constexpr int g = decltype(gc)::value;
+            if constexpr (g < 4 * KS) {
+                constexpr int qb = g / (2 * KS), which = (g / KS) & 1, ks = g % KS;
+                return rd.row(which ? dOb : Qb, qb, ks);
+            } else {
+                constexpr int qb = (g - 4 * KS) / (2 * KS), i = g % (2 * KS);
+                constexpr int sx = i / (2 * DB), db = (i / 2) % DB, which = i & 1;
+                return rd.transposed(which ? Qb : dOb, qb, sx, db);
+            }
+        };
+        auto mma = [&](auto gc, s16x8 a) __attribute__((always_inline)) {
+            constexpr int g = decltype(gc)::value;
+            if constexpr (g < 4 * KS) {
+                constexpr int qb = g / (2 * KS), which = (g / KS) & 1, ks = g % KS;
+                if constexpr (which) M::acc_v(a, vf[ks], dp[qb]);
+                else if constexpr (ks == 0) M::first_v(a, kf[0], s[qb]);
+                else M::acc_v(a, kf[ks], s[qb]);
+            } else {
+                constexpr int qb = (g - 4 * KS) / (2 * KS), i = g % (2 * KS);
+                constexpr int sx = i / (2 * DB), db = (i / 2) % DB, which = i & 1;
+                if constexpr (which) dk[db] = M::run(a, sb[2 * qb + sx], dk[db]);
+                else dv[db] = M::run(a, pb[2 * qb + sx], dv[db]);
+            }
+        };
+        auto vop = [&](auto op_) __attribute__((always_inline)) {
+            constexpr int o = decltype(op_)::value;
+            constexpr int qb = Plan::plan.op[o].blk, kind = Plan::plan.op[o].kind, e = Plan::plan.op[o].e;
+            [[maybe_unused]] constexpr int c = 32 * qb + 8 * (e >> 2) + (e & 3);
+            if constexpr (kind == 0) {
+                s[qb][e] = __builtin_fmaf(s[qb][e], sl2, -l4[qb][e >> 2][e & 3]);
+            } else if constexpr (kind == 1) {
+                const float pe = __builtin_amdgcn_exp2f(s[qb][e]);
+                if constexpr (EDGE) s[qb][e] = (c > c_hi || c < c_lo) ? 0.f : pe;
+                else s[qb][e] = pe;
+            } else if constexpr (kind == 2) {
+                if constexpr (EDGE) dp[qb][e] = (c > c_hi || c < c_lo) ? 0.f : s[qb][e] * dp[qb][e];   // (dP may be anything there)
+                else dp[qb][e] *= s[qb][e];
+            } else if constexpr (kind == 3) {
+                pb[2 * qb + (e >> 2)][(2 * e) & 7] = (T)s[qb][2 * e];
+                pb[2 * qb + (e >> 2)][((2 * e) & 7) + 1] = (T)s[qb][2 * e + 1];
+            } else {
+                sb[2 * qb + (e >> 2)][(2 * e) & 7] = (T)dp[qb][2 * e];
+                sb[2 * qb + (e >> 2)][((2 * e) & 7) + 1] = (T)dp[qb][2 * e + 1];
+            }
+        };
+        mma_stream<NSTEP, FW>(frag, mma, [&](auto gc) __attribute__((always_inline)) {
+            constexpr int g = decltype(gc)::value;
+            // this wave's pieces of tile j + 1, requested a tile ago, are confirmed before those of j + 2 go out
+            if constexpr (g == NSTEP - FW) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if constexpr (g >= NSTEP - FW && (g - (NSTEP - FW)) % PSTEP == 0) fetch_piece(next, fre, IC<(g - (NSTEP - FW)) / PSTEP>{});
+            if constexpr (g == NSTEP - 1) fetch_piece(next, fre, IC<2 * LPT>{});
+            constexpr int o0 = Plan::plan.start[g], o1 = Plan::plan.start[g + 1];
+            static_for<o1 - o0>([&](auto oc) __attribute__((always_inline)) { vop(IC<o0 + decltype(oc)::value>{}); });
+        });
+        // tile j + 1 complete, tile j released (the bare barrier: the loads just issued stay in flight)
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const int was = cur;
+        cur = nxt; nxt = fre; fre = was;
+    };
+
+    if (j0 < j1) {
+        fetch_tile(j0, 0);
+        fetch_tile(j0 + 1, 1);
+        tile_ready();
+        for (int j = j0; j < j1;) {
+            // a head's tiles: masked ones, whole ones, masked ones
+            const int g = j / nt, x = j - g * nt;
+            const bool edge = x < m0 || x >= m1;
+            const int end = min(j1, g * nt + (x < m0 ? min(m0, nt) : edge ? nt : m1));
+            if (edge) for (; j < end; ++j) tile(j, IC<1>{});
+            else for (; j < end; ++j) tile(j, IC<0>{});
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // nothing in flight into an LDS that is given up
+    }
+
+    if (krow >= w.Nk) return;
+    const int64_t out = ((int64_t)bg * w.Nk + krow) * w.d;
+    float* pk = parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 + (krow - k0)) * w.d;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int c = 32 * db + 8 * g + 4 * h;
+            if (c >= w.d) continue;
+            f32x4 xk, xv;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { xk[e] = dk[db][4 * g + e] * w.scale; xv[e] = dv[db][4 * g + e]; }
+            if (split && ns > 1) {
+                *reinterpret_cast<f32x4*>(pk + c) = xk;
+                *reinterpret_cast<f32x4*>(pk + (int64_t)128 * w.d + c) = xv;
+            } else {
+                vec4 yk, yv;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { yk[e] = (T)xk[e]; yv[e] = (T)xv[e]; }
+                *reinterpret_cast<vec4*>(dKg + out + c) = yk;
+                *reinterpret_cast<vec4*>(dVg + out + c) = yv;
+            }
+        }
+}
+
 // ---------------------------------------------------------------- the split key blocks' parts, in order
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -392,9 +809,14 @@ int launch_bwd(const void* q, const void* k, const void* v, const void* o, const
             launch_kernel(kdq, dim3((unsigned)nq), dim3(256), 0, s, static_cast<const T*>(q), static_cast<const T*>(k),
                           static_cast<const T*>(v), static_cast<const T*>(dout), st, static_cast<T*>(dq), w, p.nqp, p.rows, nqblk, (int)nq);
     };
-    if (w.d <= 64) go(window_bwd_dq_kernel<T, 64>, window_bwd_dkv_kernel<T, 64>);
-    else if (w.d <= 128) go(window_bwd_dq_kernel<T, 128>, window_bwd_dkv_kernel<T, 128>);
-    else if constexpr (sizeof(T) == 2) go(window_bwd_dq_kernel<T, 256>, window_bwd_dkv_kernel<T, 256>);
+    if constexpr (sizeof(T) == 2) {
+        if (w.d <= 64) go(window_bwd_dq16_kernel<T, 64>, window_bwd_dkv16_kernel<T, 64>);
+        else if (w.d <= 128) go(window_bwd_dq16_kernel<T, 128>, window_bwd_dkv16_kernel<T, 128>);
+        else go(window_bwd_dq_kernel<T, 256>, window_bwd_dkv_kernel<T, 256>);
+    } else {
+        if (w.d <= 64) go(window_bwd_dq_kernel<T, 64>, window_bwd_dkv_kernel<T, 64>);
+        else go(window_bwd_dq_kernel<T, 128>, window_bwd_dkv_kernel<T, 128>);
+    }
     if (p.ns > 1) {
         const int64_t n4 = (int64_t)w.B * w.Hkv * p.nsb * 2 * 128 * (w.d / 4);
         launch_kernel(window_bwd_join_kernel<T>, dim3((unsigned)cdiv(n4, 256)), dim3(256), 0, s, parts, static_cast<T*>(dk),

@@ -55,6 +55,7 @@ template <typename T, int D> struct TileReader {
     static constexpr int SUB = 8 * RB;                 // bytes of 8 rows
     static constexpr int KS = RB / 32;                 // chunk pairs of a row
     static constexpr int DB = D / 32;
+    static constexpr int COLB = sizeof(T) == 2 ? 512 : 1024;   // image bytes between 32-column blocks
     using frag = typename Frag16<T>::type;
     int rb[2], tb[2];
 
@@ -74,10 +75,19 @@ template <typename T, int D> struct TileReader {
     __device__ __forceinline__ frag row(const char* tile, int blk, int ks) const {
         return *reinterpret_cast<const frag*>(tile + rb[ks & 1] + SUB * 4 * blk + 512 * (ks >> 1));
     }
+    // 16-bit: the A operand of k-step st of block blk (rows 32 blk + 16 st + ...) and columns 32 db ..
+    __device__ __forceinline__ s16x8 transposed(const char* tile, int blk, int st, int db) const {
+        const int imm = SUB * 2 * (2 * blk + st) + COLB * db;
+        const s16x4 lo = lds_read_tr(tile + tb[0] + imm);
+        const s16x4 hi = lds_read_tr(tile + tb[1] + imm);
+        s16x8 a;
+        a[0] = lo[0]; a[1] = lo[1]; a[2] = lo[2]; a[3] = lo[3];
+        a[4] = hi[0]; a[5] = hi[1]; a[6] = hi[2]; a[7] = hi[3];
+        return a;
+    }
     // acc[db] += tile[rows of blk][32 columns of db]^T x[rows of blk], x an accumulator-shaped block
     // (rounded to T): the accumulator's row index is this product's k index, in place.  `tile` may point
     // at a later column block (COLB bytes each): acc then holds the columns from there on.
-    static constexpr int COLB = sizeof(T) == 2 ? 512 : 1024;
     template <int NDB>
     __device__ __forceinline__ void add_transposed(const char* tile, int blk, const f32x16& x, f32x16 (&acc)[NDB]) const {
         if constexpr (sizeof(T) == 2) {
@@ -88,13 +98,7 @@ template <typename T, int D> struct TileReader {
                 for (int j = 0; j < 8; ++j) b[j] = (T)x[8 * st + j];
 #pragma unroll
                 for (int db = 0; db < NDB; ++db) {
-                    const int imm = SUB * 2 * (2 * blk + st) + COLB * db;
-                    const s16x4 lo = lds_read_tr(tile + tb[0] + imm);
-                    const s16x4 hi = lds_read_tr(tile + tb[1] + imm);
-                    s16x8 a;
-                    a[0] = lo[0]; a[1] = lo[1]; a[2] = lo[2]; a[3] = lo[3];
-                    a[4] = hi[0]; a[5] = hi[1]; a[6] = hi[2]; a[7] = hi[3];
-                    acc[db] = Mma<T>::run(a, b, acc[db]);
+                    acc[db] = Mma<T>::run(transposed(tile, blk, st, db), b, acc[db]);
                 }
             }
         } else {
@@ -141,6 +145,23 @@ template <typename T, int D, int ROWS, int THREADS> struct TileFetch {
 #endif
     }
 };
+
+// A sequence of MFMAs as one software-pipelined stream: the LDS fragment of step i + FW is requested when
+// step i issues (left alone, the scheduler sinks every read to just in front of its MFMA), after(i) runs in
+// that MFMA's shadow, and the order is pinned.
+template <int N, int FW, class Frag, class Mm, class After>
+__device__ __forceinline__ void mma_stream(Frag&& frag, Mm&& mm, After&& after) {
+    decltype(frag(IC<0>{})) win[FW];
+    static_for<(FW < N ? FW : N)>([&](auto ic) __attribute__((always_inline)) { win[decltype(ic)::value] = frag(ic); });
+    static_for<N>([&](auto ic) __attribute__((always_inline)) {
+        constexpr int i = decltype(ic)::value;
+        const auto a = win[i % FW];
+        mm(ic, a);
+        if constexpr (i + FW < N) win[i % FW] = frag(IC<i + FW>{});
+        after(ic);
+        __builtin_amdgcn_sched_barrier(0);
+    });
+}
 
 // Everyone's fetches so far are complete and everyone has left the tile read before.
 __device__ __forceinline__ void tile_ready() {
