@@ -4,12 +4,11 @@
 //     dP = dO V^T,  delta = rowsum(dO o O),  dS = P o (dP - delta)
 //     dQ = scale dS K,   dK = scale dS^T Q                   dK, dV summed over the query heads that share them
 //
-// Three kernels and, where keys are split, a fourth; no atomics, so results do not depend on timing.
-//   rows    per query row: -delta and lse * log2(e), in float32, in an array padded to whole tiles whose
-//           padding and whose rows that see nothing get lse = +inf (P = 0).
+// Two kernels and, where keys are split, a third; no atomics, so results do not depend on timing.
 //   dQ      workgroup = 128 query rows (4 waves x 32) and the key tiles they see, as in the forward:
 //           S^T = K Q^T and dP^T = V dO^T put the query on the lane; dS^T is in place the B operand of
-//           dQ^T += K^T dS^T.
+//           dQ^T += K^T dS^T.  Its prologue has the rows of dO at hand, reads those of O and leaves -delta and
+//           lse * log2(e) of every row for the second kernel.
 //   dK, dV  workgroup = 128 keys (4 waves x 32) of one key/value head and, head after head of its group,
 //           the query tiles that see some of them: S = Q K^T and dP = dO V^T put the key on the lane; P and
 //           dS are in place the B operands of dV^T += dO^T P and dK^T += Q^T dS.  The sums over the group
@@ -30,67 +29,60 @@ template <typename T, int D> constexpr int bwd_tile() { return D * (int)sizeof(T
 constexpr int kStatPad = 64;                         // rows of the statistics per head: a multiple of this
 
 // ---------------------------------------------------------------- row statistics
-template <typename T>
-__global__ void __launch_bounds__(256)
-window_bwd_rows_kernel(const T* __restrict__ Og, const T* __restrict__ dOg, const float* __restrict__ LSEg,
-                       float* __restrict__ st, WindowShape w, int nqp, int64_t rows) {
+// A lane's query row of dO and O (chunks 2 ks + h): -delta and lse * log2(e) of the row, which the dK, dV kernel reads
+// from `st` (two arrays of `rows`, nqp a head).  Every row up to nqp is written; those that see nothing get
+// lse = +inf (P = 0) and delta = 0.  All lanes of the wave take part.
+struct RowStat { float lse2, ndelta; };
+template <typename T, int KS, typename Frag>
+__device__ __forceinline__ RowStat row_stat(const Frag (&of)[KS], const T* out_row, const float* lse_at, bool live, int d, int h,
+                                            float* st, int64_t rows, int64_t srow, bool store) {
     constexpr int EPC = 16 / (int)sizeof(T);
     typedef T vec __attribute__((ext_vector_type(EPC)));
-    const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);     // padded row
-    if (row >= rows) return;
-    const int64_t bh = row / nqp;
-    const int i = (int)(row - bh * nqp), b = (int)(bh / w.H);
-    const int len = w.lens ? w.lens[b] : w.Nk;
-    const bool live = i < w.Nq && i + w.Nk - w.Nq < len;
     float acc = 0.f;
     if (live) {
-        const int64_t at = (bh * w.Nq + i) * w.d;
-        for (int c = (threadIdx.x & 15) * EPC; c < w.d; c += 16 * EPC) {
-            const vec x = *reinterpret_cast<const vec*>(Og + at + c), y = *reinterpret_cast<const vec*>(dOg + at + c);
 #pragma unroll
-            for (int j = 0; j < EPC; ++j) acc += (float)x[j] * (float)y[j];
+        for (int ks = 0; ks < KS; ++ks) {
+            const int c = (2 * ks + h) * EPC;
+            if (c < d) {
+                const vec x = *reinterpret_cast<const vec*>(out_row + c), y = __builtin_bit_cast(vec, of[ks]);
+#pragma unroll
+                for (int j = 0; j < EPC; ++j) acc += (float)x[j] * (float)y[j];
+            }
         }
     }
-    acc += dpp_mov<0xB1>(acc);
-    acc += dpp_mov<0x4E>(acc);
-    acc += dpp_mov<0x141>(acc);
-    acc += dpp_mov<0x140>(acc);
-    if ((threadIdx.x & 15) == 0) {
-        st[row] = live ? LSEg[bh * w.Nq + i] * kLog2eW : INFINITY;
-        st[rows + row] = live ? -acc : 0.f;
+    acc = half_exchange_sum(acc);
+    const RowStat s{live ? *lse_at * kLog2eW : INFINITY, live ? -acc : 0.f};
+    if (store && h == 0) {
+        st[srow] = s.lse2;
+        st[rows + srow] = s.ndelta;
     }
+    return s;
 }
 
 // ---------------------------------------------------------------- dQ
 template <typename T, int D>
 __global__ void __launch_bounds__(256, D * sizeof(T) <= 256 ? 2 : 1)
 window_bwd_dq_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
-                     const T* __restrict__ dOg, const float* __restrict__ st, T* __restrict__ dQg,
-                     WindowShape w, int nqp, int64_t rows, int nqblk, int nwg) {
+                     const T* __restrict__ dOg, const T* __restrict__ Og, const float* __restrict__ LSEg, float* __restrict__ st, T* __restrict__ dQg,
+                     WindowShape w, int nqp, int64_t rows, int nqblk) {
     using R = TileReader<T, D>;
     constexpr int BN = bwd_tile<T, D>(), NB = BN / 32, TILE_B = BN * R::RB;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B];   // K0 K1 V0 V1
 
-    const int lid = xcd_range_id(blockIdx.x, nwg);
-    const int bh = lid / nqblk;
+    const Ranked at_ = ranked(blockIdx.x, w.B * w.H);
+    const int bh = at_.head, q0 = (nqblk - 1 - at_.rank) * 128;      // the last block of a head sees the most keys
     const int b = bh / w.H, head = bh - b * w.H, kvh = head / (w.H / w.Hkv);
-    const int q0 = (lid - bh * nqblk) * 128;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, h = lane >> 5;
-    const int len = w.lens ? min(max(w.lens[b], 0), w.Nk) : w.Nk;
-    const int shift = w.Nk - w.Nq;
-    const int pa = q0 + shift, pz = min(min(q0 + 128, w.Nq) + shift, len);
-    const int lo = max(0, pa - w.window + 1);
-    const int t_win = lo / BN, t_end = pz > pa ? (pz + BN - 1) / BN : t_win;
-    const int n_sink = pz > pa ? min((min(w.sinks, pz) + BN - 1) / BN, t_win) : 0;
-    const int ntiles = n_sink + (t_end - t_win);
+    const KeyTiles<BN> kt(w, b, q0, 128);
+    const int ntiles = kt.ntiles;
 
     const int qrow = q0 + 32 * wave + r;
-    const int p_own = qrow + shift;
-    const bool live = qrow < w.Nq && p_own < len;
-    const int p_hi = live ? p_own : -1, p_lo = p_own - w.window + 1;
-    const int wave_lo = q0 + 32 * wave + shift, wave_hi = min(wave_lo + 32, pz) - 1;
+    const int p_own = qrow + kt.shift;
+    const bool live = qrow < w.Nq && p_own < kt.len;
+    const RowSees sees{p_own - w.window + 1, live ? p_own : -1};
+    const int wave_lo = q0 + 32 * wave + kt.shift, wave_hi = min(wave_lo + 32, kt.pz) - 1;
 
     const T* Kh = Kg + b * w.ks[0] + kvh * w.ks[1];
     const T* Vh = Vg + b * w.vs[0] + kvh * w.vs[1];
@@ -111,17 +103,17 @@ window_bwd_dq_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T
             }
         }
     }
-    const int64_t srow = (int64_t)bh * nqp + min(qrow, nqp - 1);
-    const float lse2 = st[srow], ndelta = st[rows + srow];
+    const int64_t orow = (int64_t)bh * w.Nq + min(qrow, w.Nq - 1);
+    const RowStat stat = row_stat<T>(of, Og + orow * w.d, LSEg + orow, live, w.d, h, st, rows, (int64_t)bh * nqp + qrow, qrow < nqp);
+    const float lse2 = stat.lse2, ndelta = stat.ndelta;
     const float sl2 = w.scale * kLog2eW;
 
     const R rd(lane);
     const TileFetch<T, D, BN, 256> kfetch(tid, w.ks[2], w.d), vfetch(tid, w.vs[2], w.d);
-    auto first_key = [&](int t) __attribute__((always_inline)) { return (t < n_sink ? t : t - n_sink + t_win) * BN; };
     auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
-        const int k0 = first_key(t);
-        const bool all = k0 + BN <= pz && (k0 >= lo || k0 + BN <= w.sinks);
-        auto keep = [&](int row) { const int k = k0 + row; return (k < pz) & ((k >= lo) | (k < w.sinks)); };
+        const int k0 = kt.first_key(t);
+        const bool all = kt.all(k0, w.sinks);
+        auto keep = [&](int row) { return kt.one(k0 + row, w.sinks); };
         kfetch.fetch(Kh + (int64_t)k0 * w.ks[2], lds + buf * TILE_B, all, keep);
         vfetch.fetch(Vh + (int64_t)k0 * w.vs[2], lds + (2 + buf) * TILE_B, all, keep);
     };
@@ -134,14 +126,13 @@ window_bwd_dq_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T
 
     if (ntiles > 0) fetch(0, 0);
     for (int t = 0; t < ntiles; ++t) {
-        const int buf = t & 1, k0 = first_key(t);
+        const int buf = t & 1, k0 = kt.first_key(t);
         tile_ready();
         if (t + 1 < ntiles) fetch(t + 1, buf ^ 1);
         if (k0 > wave_hi || (k0 + BN <= wave_lo - w.window + 1 && k0 >= w.sinks)) continue;
         const char* Kb = lds + buf * TILE_B;
         const char* Vb = lds + (2 + buf) * TILE_B;
-        const bool edge = !(k0 + BN - 1 <= wave_lo && wave_lo + 31 < len && wave_lo + 31 - shift < w.Nq &&
-                            (k0 >= wave_lo + 31 - w.window + 1 || k0 + BN <= w.sinks));
+        const bool edge = !(k0 + BN - 1 <= wave_lo && wave_lo + 31 < kt.pz && (k0 >= wave_lo + 31 - w.window + 1 || k0 + BN <= w.sinks));
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb) {
             f32x16 s, dp;
@@ -153,13 +144,7 @@ window_bwd_dq_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T
             for (int ks = 0; ks < R::KS; ++ks) dp = mma_chunk<T>(rd.row(Vb, kb, ks), of[ks], dp);
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sl2, -lse2)) * dp[i];
-            if (edge) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int key = k0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (!((key <= p_hi) & ((key >= p_lo) | (key < w.sinks)))) s[i] = 0.f;
-                }
-            }
+            if (edge) sees.hide(s, kt, t, k0, k0 + 32 * kb + 4 * h, w.sinks, 0.f);
             rd.add_transposed(Kb, kb, s, dq);
         }
     }
@@ -189,51 +174,44 @@ window_bwd_dq_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 2)
 window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
-                       const T* __restrict__ dOg, const float* __restrict__ st, T* __restrict__ dQg,
-                       WindowShape w, int nqp, int64_t rows, int nqblk, int nwg) {
+                       const T* __restrict__ dOg, const T* __restrict__ Og, const float* __restrict__ LSEg, float* __restrict__ st, T* __restrict__ dQg,
+                       WindowShape w, int nqp, int64_t rows, int nqblk) {
     using M = Mma<T>;
     using R = TileReader<T, D>;
     constexpr int BN = 64, KS = R::KS, DB = R::DB, TILE_B = BN * R::RB, FW = 4;
     __shared__ __attribute__((aligned(1024))) char lds[5 * TILE_B];   // K0 K1 K2 V0 V1
 
-    const int lid = xcd_range_id(blockIdx.x, nwg);
-    const int bh = lid / nqblk;
+    const Ranked at_ = ranked(blockIdx.x, w.B * w.H);
+    const int bh = at_.head, q0 = (nqblk - 1 - at_.rank) * 128;      // the last block of a head sees the most keys
     const int b = bh / w.H, head = bh - b * w.H, kvh = head / (w.H / w.Hkv);
-    const int q0 = (lid - bh * nqblk) * 128;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, h = lane >> 5;
-    const int len = w.lens ? min(max(w.lens[b], 0), w.Nk) : w.Nk;
-    const int shift = w.Nk - w.Nq;
-    const int pa = q0 + shift, pz = min(min(q0 + 128, w.Nq) + shift, len);
-    const int lo = max(0, pa - w.window + 1);
-    const int t_win = lo / BN, t_end = pz > pa ? (pz + BN - 1) / BN : t_win;
-    const int n_sink = pz > pa ? min((min(w.sinks, pz) + BN - 1) / BN, t_win) : 0;
-    const int ntiles = n_sink + (t_end - t_win);
+    const KeyTiles<BN> kt(w, b, q0, 128);
+    const int ntiles = kt.ntiles;
 
     const int qrow = q0 + 32 * wave + r;
-    const int p_own = qrow + shift;
-    const bool live = qrow < w.Nq && p_own < len;
-    const int p_hi = live ? p_own : -1, p_lo = p_own - w.window + 1;
-    const int wave_lo = q0 + 32 * wave + shift, wave_hi = min(wave_lo + 32, pz) - 1;
+    const int p_own = qrow + kt.shift;
+    const bool live = qrow < w.Nq && p_own < kt.len;
+    const RowSees sees{p_own - w.window + 1, live ? p_own : -1};
+    const int wave_lo = q0 + 32 * wave + kt.shift, wave_hi = min(wave_lo + 32, kt.pz) - 1;
 
     const T* Kh = Kg + b * w.ks[0] + kvh * w.ks[1];
     const T* Vh = Vg + b * w.vs[0] + kvh * w.vs[1];
     const R rd(lane);
     const TileFetch<T, D, BN, 256> kfetch(tid, w.ks[2], w.d), vfetch(tid, w.vs[2], w.d);
-    auto first_key = [&](int t) __attribute__((always_inline)) { return (t < n_sink ? t : t - n_sink + t_win) * BN; };
     auto fetch = [&](int t, int kslot) __attribute__((always_inline)) {
         if (t >= ntiles) return;
-        const int k0 = first_key(t);
-        char* kt = lds + kslot * TILE_B;
-        char* vt = lds + (3 + (t & 1)) * TILE_B;
-        if (k0 + BN <= pz && (k0 >= lo || k0 + BN <= w.sinks)) {
-            kfetch.fetch(Kh + (int64_t)k0 * w.ks[2], kt, true, [](int) { return true; });
-            vfetch.fetch(Vh + (int64_t)k0 * w.vs[2], vt, true, [](int) { return true; });
+        const int k0 = kt.first_key(t);
+        char* kd = lds + kslot * TILE_B;
+        char* vd = lds + (3 + (t & 1)) * TILE_B;
+        if (kt.all(k0, w.sinks)) {
+            kfetch.fetch(Kh + (int64_t)k0 * w.ks[2], kd, true, [](int) { return true; });
+            vfetch.fetch(Vh + (int64_t)k0 * w.vs[2], vd, true, [](int) { return true; });
         } else {
-            auto keep = [&](int row) { const int k = k0 + row; return (k < pz) & ((k >= lo) | (k < w.sinks)); };
-            kfetch.fetch(Kh + (int64_t)k0 * w.ks[2], kt, false, keep);
-            vfetch.fetch(Vh + (int64_t)k0 * w.vs[2], vt, false, keep);
+            auto keep = [&](int row) { return kt.one(k0 + row, w.sinks); };
+            kfetch.fetch(Kh + (int64_t)k0 * w.ks[2], kd, false, keep);
+            vfetch.fetch(Vh + (int64_t)k0 * w.vs[2], vd, false, keep);
         }
     };
     fetch(0, 0);
@@ -255,8 +233,9 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
             }
         }
     }
-    const int64_t srow = (int64_t)bh * nqp + min(qrow, nqp - 1);
-    const float lse2 = st[srow], ndelta = st[rows + srow];
+    const int64_t orow = (int64_t)bh * w.Nq + min(qrow, w.Nq - 1);
+    const RowStat stat = row_stat<T>(of, Og + orow * w.d, LSEg + orow, live, w.d, h, st, rows, (int64_t)bh * nqp + qrow, qrow < nqp);
+    const float lse2 = stat.lse2, ndelta = stat.ndelta;
     const float sl2 = w.scale * kLog2eW;
 
     f32x16 dq[DB];
@@ -268,25 +247,18 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
 
     int cur = 0, nxt = 1, fre = 2;                 // K slots of tiles t, t + 1, t + 2
     for (int t = 0; t < ntiles; ++t) {
-        const int k0 = first_key(t);
+        const int k0 = kt.first_key(t);
         const char* Kb = lds + cur * TILE_B;
         const char* Vb = lds + (3 + (t & 1)) * TILE_B;
         const bool some = !(k0 > wave_hi || (k0 + BN <= wave_lo - w.window + 1 && k0 >= w.sinks));
-        const bool edge = !(k0 + BN - 1 <= wave_lo && wave_lo + 31 < len && wave_lo + 31 - shift < w.Nq &&
-                            (k0 >= wave_lo + 31 - w.window + 1 || k0 + BN <= w.sinks));
+        const bool edge = !(k0 + BN - 1 <= wave_lo && wave_lo + 31 < kt.pz && (k0 >= wave_lo + 31 - w.window + 1 || k0 + BN <= w.sinks));
         f32x16 s[2], dp[2];
         typename M::vec8 sb[4];
         auto pds = [&](int kb, int i) __attribute__((always_inline)) {
             s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], sl2, -lse2)) * (dp[kb][i] + ndelta);
         };
         auto finish = [&](int kb) __attribute__((always_inline)) {
-            if (edge) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int key = k0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (!((key <= p_hi) & ((key >= p_lo) | (key < w.sinks)))) s[kb][i] = 0.f;
-                }
-            }
+            if (edge) sees.hide(s[kb], kt, t, k0, k0 + 32 * kb + 4 * h, w.sinks, 0.f);
 #pragma unroll
             for (int i = 0; i < 16; ++i) sb[2 * kb + (i >> 3)][i & 7] = (T)s[kb][i];
         };
@@ -364,17 +336,17 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256, D * sizeof(T) <= 128 ? 2 : 1)
 window_bwd_dkv_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
                       const T* __restrict__ dOg, const float* __restrict__ st, T* __restrict__ dKg, T* __restrict__ dVg,
-                      float* __restrict__ parts, WindowShape w, int nqp, int64_t rows, int nkblk, int nsb, int ns, int nwg) {
+                      float* __restrict__ parts, WindowShape w, int nqp, int64_t rows, int nsb, int ns) {
     using R = TileReader<T, D>;
     constexpr int BQ = bwd_tile<T, D>(), NB = BQ / 32, TILE_B = BQ * R::RB;
     constexpr int ODB = R::DB < 4 ? R::DB : 4, NC = R::DB / ODB;             // column blocks kept, workgroups per key block
     __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B + 4 * 64 * 4];   // Q0 Q1 dO0 dO1 [buf][lse2 | -delta][64]
     float* stat = reinterpret_cast<float*>(lds + 4 * TILE_B);
 
-    // a head's units: the split sink blocks first (the longest), then the other key blocks
-    const int units = nsb * ns + (nkblk - nsb);
-    const int lidc = xcd_range_id(blockIdx.x, nwg), lid = lidc / NC, col0 = (lidc - lid * NC) * ODB * 32;
-    const int bg = lid / units, unit = lid - bg * units;
+    // a head's units: the split sink blocks first, then the other key blocks; the last ones see the fewest queries
+    const int lid = blockIdx.x / NC, col0 = ((int)blockIdx.x - lid * NC) * ODB * 32;
+    const Ranked at_ = ranked(lid, w.B * w.Hkv);
+    const int bg = at_.head, unit = at_.rank;
     const bool split = unit < nsb * ns;
     const int kblk = split ? unit / ns : unit - nsb * ns + nsb, part = split ? unit - kblk * ns : 0, nparts = split ? ns : 1;
     const int b = bg / w.Hkv, kvh = bg - b * w.Hkv, group = w.H / w.Hkv;
@@ -517,7 +489,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256, 1)
 window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
                         const T* __restrict__ dOg, const float* __restrict__ st, T* __restrict__ dKg, T* __restrict__ dVg,
-                        float* __restrict__ parts, WindowShape w, int nqp, int64_t rows, int nkblk, int nsb, int ns, int nwg) {
+                        float* __restrict__ parts, WindowShape w, int nqp, int64_t rows, int nsb, int ns) {
     using M = Mma<T>;
     using vec8 = typename M::vec8;
     using vec4 = typename M::vec4;
@@ -528,9 +500,8 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
     __shared__ __attribute__((aligned(1024))) char lds[6 * TILE_B + 6 * BQ * 4];    // Q0 Q1 Q2 dO0 dO1 dO2, [buf][lse2 | -delta][64]
     float* stat = reinterpret_cast<float*>(lds + 6 * TILE_B);
 
-    const int units = nsb * ns + (nkblk - nsb);
-    const int lid = xcd_range_id(blockIdx.x, nwg);
-    const int bg = lid / units, unit = lid - bg * units;
+    const Ranked at_ = ranked(blockIdx.x, w.B * w.Hkv);
+    const int bg = at_.head, unit = at_.rank;
     const bool split = unit < nsb * ns;
     const int kblk = split ? unit / ns : unit - nsb * ns + nsb, part = split ? unit - kblk * ns : 0, nparts = split ? ns : 1;
     const int b = bg / w.Hkv, kvh = bg - b * w.Hkv, group = w.H / w.Hkv;
@@ -796,18 +767,17 @@ int launch_bwd(const void* q, const void* k, const void* v, const void* o, const
     float* parts = ws + p.stat_floats;
     const int nqblk = (int)cdiv(w.Nq, 128);
     const int64_t nq = (int64_t)w.B * w.H * nqblk, nkv = (int64_t)w.B * w.Hkv * (p.nsb * (int64_t)p.ns + p.nkblk - p.nsb) * (w.d > 128 ? 2 : 1);
-    if (nq > 0x7fffffff || nkv > 0x7fffffff || cdiv(p.rows, 16) > 0x7fffffff)
+    if (nq > 0x7fffffff || nkv > 0x7fffffff)
         return fail(MYFA_E_UNSUPPORTED, "window attention backward: too many blocks");
-    if (p.rows > 0)
-        launch_kernel(window_bwd_rows_kernel<T>, dim3((unsigned)cdiv(p.rows, 16)), dim3(256), 0, s, static_cast<const T*>(o),
-                      static_cast<const T*>(dout), lse, st, w, p.nqp, p.rows);
     auto go = [&](auto kdq, auto kdkv) {
-        launch_kernel(kdkv, dim3((unsigned)nkv), dim3(256), 0, s, static_cast<const T*>(q), static_cast<const T*>(k),
-                      static_cast<const T*>(v), static_cast<const T*>(dout), st, static_cast<T*>(dk), static_cast<T*>(dv), parts,
-                      w, p.nqp, p.rows, p.nkblk, p.nsb, p.ns, (int)nkv);
+        // (dQ first: it leaves the row statistics that dK, dV reads)
         if (nq > 0)
             launch_kernel(kdq, dim3((unsigned)nq), dim3(256), 0, s, static_cast<const T*>(q), static_cast<const T*>(k),
-                          static_cast<const T*>(v), static_cast<const T*>(dout), st, static_cast<T*>(dq), w, p.nqp, p.rows, nqblk, (int)nq);
+                          static_cast<const T*>(v), static_cast<const T*>(dout), static_cast<const T*>(o), lse, st, static_cast<T*>(dq),
+                          w, p.nqp, p.rows, nqblk);
+        launch_kernel(kdkv, dim3((unsigned)nkv), dim3(256), 0, s, static_cast<const T*>(q), static_cast<const T*>(k),
+                      static_cast<const T*>(v), static_cast<const T*>(dout), st, static_cast<T*>(dk), static_cast<T*>(dv), parts,
+                      w, p.nqp, p.rows, p.nsb, p.ns);
     };
     if constexpr (sizeof(T) == 2) {
         if (w.d <= 64) go(window_bwd_dq16_kernel<T, 64>, window_bwd_dkv16_kernel<T, 64>);

@@ -33,6 +33,8 @@ constexpr float kLn2W = 0.6931471805599453f;
 constexpr int kOffPast = 0x7FFF0000;
 constexpr int kTileBytesMax = 0x7FFE0000;
 
+__device__ __forceinline__ constexpr int cdiv32(int a, int b) { return (a + b - 1) / b; }
+
 template <typename T> struct Frag16 { using type = s16x8; };
 template <> struct Frag16<float> { using type = f32x4; };
 
@@ -153,6 +155,7 @@ template <int N, int FW, class Frag, class Mm, class After>
 __device__ __forceinline__ void mma_stream(Frag&& frag, Mm&& mm, After&& after) {
     decltype(frag(IC<0>{})) win[FW];
     static_for<(FW < N ? FW : N)>([&](auto ic) __attribute__((always_inline)) { win[decltype(ic)::value] = frag(ic); });
+    __builtin_amdgcn_s_setprio(1);      // the matrix pipe first: 3 % on the forward, 1 % on the backward
     static_for<N>([&](auto ic) __attribute__((always_inline)) {
         constexpr int i = decltype(ic)::value;
         const auto a = win[i % FW];
@@ -161,6 +164,7 @@ __device__ __forceinline__ void mma_stream(Frag&& frag, Mm&& mm, After&& after) 
         after(ic);
         __builtin_amdgcn_sched_barrier(0);
     });
+    __builtin_amdgcn_s_setprio(0);
 }
 
 // Everyone's fetches so far are complete and everyone has left the tile read before.
@@ -170,12 +174,66 @@ __device__ __forceinline__ void tile_ready() {
     asm volatile("" ::: "memory");
 }
 
-// Consecutive logical ids share keys and values; every XCD (workgroup id mod 8) gets a contiguous range
-// of them, so that what they share stays in its L2.  Speed only.
-__device__ __forceinline__ int xcd_range_id(int bid, int n) {
-    const int xcd = bid & 7, idx = bid >> 3, q = n >> 3, rr = n & 7;
-    return (xcd < rr ? xcd * (q + 1) : rr * (q + 1) + (xcd - rr) * q) + idx;
+// Which query block or unit of keys, and which head, a workgroup takes: rank 0 of every head first.  The launchers
+// rank by length, so the short ones fill the end of the launch.  Workgroups go to the XCDs round robin (id mod 8);
+// the heads are dealt such that neighbouring ones, which share keys and values, land on one XCD's L2.  Speed only.
+struct Ranked { int head, rank; };
+__device__ __forceinline__ Ranked ranked(int bid, int heads) {
+    const int rank = bid / heads, j = bid - rank * heads;
+    return {heads % 8 == 0 ? (j & 7) * (heads >> 3) + (j >> 3) : j, rank};
 }
+
+// The keys that `rows` query rows from q0 on see, as tiles of BN keys: n_sink tiles that hold sinks and nothing of any
+// window, then those from t_win on.
+template <int BN> struct KeyTiles {
+    int len, shift, pa, pz, lo, t_win, n_sink, ntiles;      // [pa, pz): the positions of rows that see anything
+    __device__ __forceinline__ KeyTiles(const WindowShape& w, int b, int q0, int rows) {
+        len = w.lens ? min(max(w.lens[b], 0), w.Nk) : w.Nk;
+        shift = w.Nk - w.Nq;
+        pa = q0 + shift;
+        pz = min(min(q0 + rows, w.Nq) + shift, len);
+        lo = max(0, pa - w.window + 1);
+        t_win = lo / BN;
+        const int t_end = pz > pa ? (pz + BN - 1) / BN : t_win;
+        n_sink = pz > pa ? min((min(w.sinks, pz) + BN - 1) / BN, t_win) : 0;
+        ntiles = n_sink + (t_end - t_win);
+    }
+    __device__ __forceinline__ int first_key(int t) const { return (t < n_sink ? t : t - n_sink + t_win) * BN; }
+    // every key of the tile is seen by some row (for the fetch), or key k is
+    __device__ __forceinline__ bool all(int k0, int sinks) const { return k0 + BN <= pz && (k0 >= lo || k0 + BN <= sinks); }
+    __device__ __forceinline__ bool one(int k, int sinks) const { return (k < pz) & ((k >= lo) | (k < sinks)); }
+    // the tiles [f0, f1) are seen whole by all `rows` rows
+    __device__ __forceinline__ int whole_from(int window, int rows) const {
+        return max(n_sink + (max(pa + rows - window, 0) + BN - 1) / BN - t_win, n_sink);
+    }
+    __device__ __forceinline__ int whole_to(int rows) const { return pz == pa + rows ? n_sink + (pa + 1) / BN - t_win : 0; }
+};
+
+// Hides from a lane's row what it does not see of a 32-key block whose accumulator element i is key
+// base + 8 (i >> 2) + (i & 3) (base: the block's first key + 4 h).  In a tile that holds only sinks, only keys behind
+// them, or one whose row's window reaches the sinks, what it sees is one range: a subtraction, a comparison and
+// a select per element.
+struct RowSees {
+    int p_lo, p_hi;                                          // the row's window; p_hi = -1: a row that sees nothing
+    template <int BN>
+    __device__ __forceinline__ void hide(f32x16& s, const KeyTiles<BN>& kt, int t, int k0, int base, int sinks, float fill) const {
+        const bool sink_tile = t < kt.n_sink;
+        if (sink_tile || k0 >= sinks) {
+            const int lo = sink_tile ? 0 : p_lo, hi = sink_tile ? min(p_hi, sinks - 1) : p_hi;
+            const int from = hi < 0 ? 1 << 30 : lo - base;
+            const unsigned span = hi < 0 ? 0u : (unsigned)(hi - lo);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if ((unsigned)(8 * (i >> 2) + (i & 3) - from) > span) s[i] = fill;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = base + 8 * (i >> 2) + (i & 3);
+                if (!((key <= p_hi) & ((key >= p_lo) | (key < sinks)))) s[i] = fill;
+            }
+        }
+    }
+};
 
 }  // namespace
 }  // namespace myfa

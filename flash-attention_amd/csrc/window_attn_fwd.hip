@@ -23,33 +23,25 @@ template <typename T, int D> constexpr int win_tile() { return D * (int)sizeof(T
 template <typename T, int D>
 __global__ void __launch_bounds__(256, D * sizeof(T) <= 256 ? 2 : 1)
 window_attn_fwd_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
-                       T* __restrict__ Og, float* __restrict__ LSEg, WindowShape w, int nqblk, int nwg) {
+                       T* __restrict__ Og, float* __restrict__ LSEg, WindowShape w, int nqblk) {
     using R = TileReader<T, D>;
     constexpr int BN = win_tile<T, D>(), NB = BN / 32, TILE_B = BN * R::RB;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B];   // K0 K1 V0 V1
 
-    const int lid = xcd_range_id(blockIdx.x, nwg);
-    const int bh = lid / nqblk;
+    const Ranked at_ = ranked(blockIdx.x, w.B * w.H);
+    const int bh = at_.head, q0 = (nqblk - 1 - at_.rank) * 128;      // the last block of a head sees the most keys
     const int b = bh / w.H, head = bh - b * w.H, kvh = head / (w.H / w.Hkv);
-    const int q0 = (lid - bh * nqblk) * 128;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, h = lane >> 5;
-    const int len = w.lens ? min(max(w.lens[b], 0), w.Nk) : w.Nk;
-    const int shift = w.Nk - w.Nq;
-
-    // positions of the workgroup's rows that see anything: [pa, pz)
-    const int pa = q0 + shift, pz = min(min(q0 + 128, w.Nq) + shift, len);
-    const int lo = max(0, pa - w.window + 1);                       // first key of the block's windows
-    const int t_win = lo / BN, t_end = pz > pa ? (pz + BN - 1) / BN : t_win;
-    const int n_sink = pz > pa ? min((min(w.sinks, pz) + BN - 1) / BN, t_win) : 0;
-    const int ntiles = n_sink + (t_end - t_win);
+    const KeyTiles<BN> kt(w, b, q0, 128);
+    const int ntiles = kt.ntiles;
 
     const int qrow = q0 + 32 * wave + r;
-    const int p_own = qrow + shift;
-    const bool live = qrow < w.Nq && p_own < len;
-    const int p_hi = live ? p_own : -1, p_lo = p_own - w.window + 1;
-    const int wave_lo = q0 + 32 * wave + shift, wave_hi = min(wave_lo + 32, pz) - 1;    // positions of the wave's live rows
+    const int p_own = qrow + kt.shift;
+    const bool live = qrow < w.Nq && p_own < kt.len;
+    const RowSees sees{p_own - w.window + 1, live ? p_own : -1};
+    const int wave_lo = q0 + 32 * wave + kt.shift, wave_hi = min(wave_lo + 32, kt.pz) - 1;    // positions of the wave's live rows
 
     const T* Kh = Kg + b * w.ks[0] + kvh * w.ks[1];
     const T* Vh = Vg + b * w.vs[0] + kvh * w.vs[1];
@@ -68,11 +60,10 @@ window_attn_fwd_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
 
     const R rd(lane);
     const TileFetch<T, D, BN, 256> kfetch(tid, w.ks[2], w.d), vfetch(tid, w.vs[2], w.d);
-    auto first_key = [&](int t) __attribute__((always_inline)) { return (t < n_sink ? t : t - n_sink + t_win) * BN; };
     auto fetch = [&](int t, int buf) __attribute__((always_inline)) {
-        const int k0 = first_key(t);
-        const bool all = k0 + BN <= pz && (k0 >= lo || k0 + BN <= w.sinks);
-        auto keep = [&](int row) { const int k = k0 + row; return (k < pz) & ((k >= lo) | (k < w.sinks)); };
+        const int k0 = kt.first_key(t);
+        const bool all = kt.all(k0, w.sinks);
+        auto keep = [&](int row) { return kt.one(k0 + row, w.sinks); };
         kfetch.fetch(Kh + (int64_t)k0 * w.ks[2], lds + buf * TILE_B, all, keep);
         vfetch.fetch(Vh + (int64_t)k0 * w.vs[2], lds + (2 + buf) * TILE_B, all, keep);
     };
@@ -87,7 +78,7 @@ window_attn_fwd_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
 
     if (ntiles > 0) fetch(0, 0);
     for (int t = 0; t < ntiles; ++t) {
-        const int buf = t & 1, k0 = first_key(t);
+        const int buf = t & 1, k0 = kt.first_key(t);
         tile_ready();
         if (t + 1 < ntiles) fetch(t + 1, buf ^ 1);
         // nothing of this tile is seen by the wave's rows
@@ -104,15 +95,9 @@ window_attn_fwd_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
             for (int ks = 0; ks < R::KS; ++ks) s[kb] = mma_chunk<T>(rd.row(Kb, kb, ks), qf[ks], s[kb]);
         }
         // every row of the wave sees every key of the tile, or a select per element
-        if (!(k0 + BN - 1 <= wave_lo && wave_lo + 31 < len && wave_lo + 31 - shift < w.Nq &&
-              (k0 >= wave_lo + 31 - w.window + 1 || k0 + BN <= w.sinks))) {
+        if (!(k0 + BN - 1 <= wave_lo && wave_lo + 31 < kt.pz && (k0 >= wave_lo + 31 - w.window + 1 || k0 + BN <= w.sinks))) {
 #pragma unroll
-            for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int key = k0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (!((key <= p_hi) & ((key >= p_lo) | (key < w.sinks)))) s[kb][i] = -INFINITY;
-                }
+            for (int kb = 0; kb < NB; ++kb) sees.hide(s[kb], kt, t, k0, k0 + 32 * kb + 4 * h, w.sinks, -INFINITY);
         }
 
         float tmax = s[0][0];
@@ -168,49 +153,46 @@ window_attn_fwd_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
 //   V(t - 1), so that two buffers of each do.  Their successors, V(t + 1) and K(t + 2), are requested behind the
 //   tile's last transposing read: hipcc makes such a read wait for every LDS-DMA load in flight, and so they have
 //   the whole of the next S and softmax to arrive in.
-//   Both products run as pinned streams (mma_stream).  The running maximum moves only when some row's grows by
-//   more than 2^8 (a vote of the wave): until then weights up to 2^8 stand in P, rounded with the same relative
-//   error, and the rescale of O, 64 multiplications a lane, stays out of most tiles.
+//   Both products run as pinned streams (mma_stream).  The weights of a tile are formed against the running maximum
+//   as it stands; only when a lane's sum passes 2^8 (a vote of the wave; its first keys always do) is the tile's
+//   maximum looked for, the running one moved, O and l rescaled and the weights formed again from the logits.
+//   Weights up to 2^8 are rounded with the same relative error, and neither the search for the maximum nor the
+//   rescale of O, 64 multiplications a lane, is in most tiles.
+//   The tiles that every row of the workgroup sees whole run in a loop without masks, bounds or tile arithmetic.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 2)
 window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
-                         T* __restrict__ Og, float* __restrict__ LSEg, WindowShape w, int nqblk, int nwg) {
+                         T* __restrict__ Og, float* __restrict__ LSEg, WindowShape w, int nqblk) {
     using M = Mma<T>;
     using R = TileReader<T, D>;
     constexpr int BN = 64, KS = R::KS, DB = R::DB, TILE_B = BN * R::RB, FW = D == 128 ? 8 : 4;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TILE_B];   // K0 K1 V0 V1
 
-    const int lid = xcd_range_id(blockIdx.x, nwg);
-    const int bh = lid / nqblk;
+    const Ranked at_ = ranked(blockIdx.x, w.B * w.H);
+    const int bh = at_.head, q0 = (nqblk - 1 - at_.rank) * 128;      // the last block of a head sees the most keys
     const int b = bh / w.H, head = bh - b * w.H, kvh = head / (w.H / w.Hkv);
-    const int q0 = (lid - bh * nqblk) * 128;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = lane & 31, h = lane >> 5;
-    const int len = w.lens ? min(max(w.lens[b], 0), w.Nk) : w.Nk;
-    const int shift = w.Nk - w.Nq;
-    const int pa = q0 + shift, pz = min(min(q0 + 128, w.Nq) + shift, len);
-    const int lo = max(0, pa - w.window + 1);
-    const int t_win = lo / BN, t_end = pz > pa ? (pz + BN - 1) / BN : t_win;
-    const int n_sink = pz > pa ? min((min(w.sinks, pz) + BN - 1) / BN, t_win) : 0;
-    const int ntiles = n_sink + (t_end - t_win);
+    const KeyTiles<BN> kt(w, b, q0, 128);
+    const int ntiles = kt.ntiles;
+    const int f0 = kt.whole_from(w.window, 128), f1 = kt.whole_to(128);      // tiles that all rows see whole
 
     const int qrow = q0 + 32 * wave + r;
-    const int p_own = qrow + shift;
-    const bool live = qrow < w.Nq && p_own < len;
-    const int p_hi = live ? p_own : -1, p_lo = p_own - w.window + 1;
-    const int wave_lo = q0 + 32 * wave + shift, wave_hi = min(wave_lo + 32, pz) - 1;
+    const int p_own = qrow + kt.shift;
+    const bool live = qrow < w.Nq && p_own < kt.len;
+    const RowSees sees{p_own - w.window + 1, live ? p_own : -1};
+    const int wave_lo = q0 + 32 * wave + kt.shift, wave_hi = min(wave_lo + 32, kt.pz) - 1;
 
     const T* Kh = Kg + b * w.ks[0] + kvh * w.ks[1];
     const T* Vh = Vg + b * w.vs[0] + kvh * w.vs[1];
     const R rd(lane);
     const TileFetch<T, D, BN, 256> kfetch(tid, w.ks[2], w.d), vfetch(tid, w.vs[2], w.d);
-    auto first_key = [&](int t) __attribute__((always_inline)) { return (t < n_sink ? t : t - n_sink + t_win) * BN; };
     auto fetch = [&](const auto& f, const T* base, int64_t stride, int t, char* to) __attribute__((always_inline)) {
-        const int k0 = first_key(t);
-        const bool all = k0 + BN <= pz && (k0 >= lo || k0 + BN <= w.sinks);
+        const int k0 = kt.first_key(t);
+        const bool all = kt.all(k0, w.sinks);
         if (all) f.fetch(base + (int64_t)k0 * stride, to, true, [](int) { return true; });
-        else f.fetch(base + (int64_t)k0 * stride, to, false, [&](int row) { const int k = k0 + row; return (k < pz) & ((k >= lo) | (k < w.sinks)); });
+        else f.fetch(base + (int64_t)k0 * stride, to, false, [&](int row) { return kt.one(k0 + row, w.sinks); });
     };
     auto fetch_k = [&](int t) __attribute__((always_inline)) { if (t < ntiles) fetch(kfetch, Kh, w.ks[2], t, lds + (t & 1) * TILE_B); };
     auto fetch_v = [&](int t) __attribute__((always_inline)) { if (t < ntiles) fetch(vfetch, Vh, w.vs[2], t, lds + (2 + (t & 1)) * TILE_B); };
@@ -235,82 +217,109 @@ window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
         for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
     float m = -INFINITY, l = 0.f;
     const float sl2 = w.scale * kLog2eW;
-    tile_ready();
+    typename M::vec8 pb[4];
 
-    for (int t = 0; t < ntiles; ++t) {
-        const int k0 = first_key(t);
-        const char* Kb = lds + (t & 1) * TILE_B;
-        const char* Vb = lds + (2 + (t & 1)) * TILE_B;
-        // something of this tile is seen by the wave's rows
-        const bool some = !(k0 > wave_hi || (k0 + BN <= wave_lo - w.window + 1 && k0 >= w.sinks));
-        typename M::vec8 pb[4];
-        if (some) {
-            f32x16 s[2];
+    auto logits = [&](const char* Kb, f32x16 (&s)[2]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
-            mma_stream<2 * KS, FW>([&](auto ic) __attribute__((always_inline)) { constexpr int i = decltype(ic)::value; return rd.row(Kb, i / KS, i % KS); },
-                                   [&](auto ic, s16x8 a) __attribute__((always_inline)) {
-                                       constexpr int i = decltype(ic)::value;
-                                       s[i / KS] = mma_chunk<T>(a, qf[i % KS], s[i / KS]);
-                                   }, [](auto) {});
-            if (!(k0 + BN - 1 <= wave_lo && wave_lo + 31 < len && wave_lo + 31 - shift < w.Nq &&
-                  (k0 >= wave_lo + 31 - w.window + 1 || k0 + BN <= w.sinks))) {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int key = k0 + 32 * kb + 8 * (i >> 2) + 4 * h + (i & 3);
-                        if (!((key <= p_hi) & ((key >= p_lo) | (key < w.sinks)))) s[kb][i] = -INFINITY;
-                    }
-            }
-            float a = vmax3(s[0][0], s[0][1], s[0][2]), c = vmax3(s[1][0], s[1][1], s[1][2]);
-#pragma unroll
-            for (int i = 3; i < 15; i += 2) { a = vmax3(a, s[0][i], s[0][i + 1]); c = vmax3(c, s[1][i], s[1][i + 1]); }
-            const float tmax = half_exchange_max(vmax3(a, c, vmax2(s[0][15], s[1][15]))) * sl2;
-            // (a row that has seen nothing has m = -inf: any key it sees moves it)
-            if (__builtin_amdgcn_ballot_w64(tmax - m > 8.f) != 0) {
-                const float m_new = fmaxf(m, tmax);
-                const float alpha = m_new == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
-                m = m_new;
-                l *= alpha;
-#pragma unroll
-                for (int db = 0; db < DB; ++db)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
-            }
-            const float ref = m == -INFINITY ? 0.f : m;
-            float sum[2] = {0.f, 0.f};
+            for (int i = 0; i < 16; ++i) s[kb][i] = 0.f;
+        mma_stream<2 * KS, FW>([&](auto ic) __attribute__((always_inline)) { constexpr int i = decltype(ic)::value; return rd.row(Kb, i / KS, i % KS); },
+                               [&](auto ic, s16x8 a) __attribute__((always_inline)) {
+                                   constexpr int i = decltype(ic)::value;
+                                   s[i / KS] = mma_chunk<T>(a, qf[i % KS], s[i / KS]);
+                               }, [](auto) {});
+    };
+    auto softmax = [&](f32x16 (&s)[2]) __attribute__((always_inline)) {
+        float sum[2];
+        auto weights = [&](float ref) __attribute__((always_inline)) {
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], sl2, -ref));
-                    sum[kb] += p;
+                    sum[kb] = i == 0 ? p : sum[kb] + p;
                     pb[2 * kb + (i >> 3)][i & 7] = (T)p;
                 }
-            l += sum[0] + sum[1];
+        };
+        weights(m == -INFINITY ? 0.f : m);
+        // (negated: a NaN or an infinite sum goes back too)
+        if (__builtin_amdgcn_ballot_w64(!(sum[0] + sum[1] <= 256.f) || m == -INFINITY) != 0) {
+            float a = vmax3(s[0][0], s[0][1], s[0][2]), c = vmax3(s[1][0], s[1][1], s[1][2]);
+#pragma unroll
+            for (int i = 3; i < 15; i += 2) { a = vmax3(a, s[0][i], s[0][i + 1]); c = vmax3(c, s[1][i], s[1][i + 1]); }
+            const float m_new = fmaxf(m, half_exchange_max(vmax3(a, c, vmax2(s[0][15], s[1][15]))) * sl2);
+            const float alpha = m_new == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);    // (nothing seen yet: all is 0)
+            m = m_new;
+            l *= alpha;
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
+            weights(m == -INFINITY ? 0.f : m);
         }
-        tile_ready();
-        constexpr int NP = 4 * DB;
-        if (some) {
-            mma_stream<NP, FW>([&](auto ic) __attribute__((always_inline)) {
-                                   constexpr int i = decltype(ic)::value, st = i / DB;
-                                   return rd.transposed(Vb, st >> 1, st & 1, i % DB);
-                               },
-                               [&](auto ic, s16x8 a) __attribute__((always_inline)) {
-                                   constexpr int i = decltype(ic)::value;
-                                   o[i % DB] = M::run(a, pb[i / DB], o[i % DB]);
-                               },
-                               [&](auto ic) __attribute__((always_inline)) {
-                                   if constexpr (decltype(ic)::value == NP - FW) { fetch_v(t + 1); fetch_k(t + 2); }
-                               });
-        } else {
-            fetch_v(t + 1);
-            fetch_k(t + 2);
+        l += sum[0] + sum[1];
+    };
+    constexpr int NP = 4 * DB;
+    auto add_pv = [&](const char* Vb, auto&& behind) __attribute__((always_inline)) {
+        mma_stream<NP, FW>([&](auto ic) __attribute__((always_inline)) {
+                               constexpr int i = decltype(ic)::value, st = i / DB;
+                               return rd.transposed(Vb, st >> 1, st & 1, i % DB);
+                           },
+                           [&](auto ic, s16x8 a) __attribute__((always_inline)) {
+                               constexpr int i = decltype(ic)::value;
+                               o[i % DB] = M::run(a, pb[i / DB], o[i % DB]);
+                           },
+                           [&](auto ic) __attribute__((always_inline)) {
+                               if constexpr (decltype(ic)::value == NP - FW) behind();
+                           });
+    };
+    tile_ready();
+
+    auto masked_tiles = [&](int t0, int t1) __attribute__((always_inline)) {
+        for (int t = t0; t < t1; ++t) {
+            const int k0 = kt.first_key(t);
+            // something of this tile is seen by the wave's rows
+            const bool some = !(k0 > wave_hi || (k0 + BN <= wave_lo - w.window + 1 && k0 >= w.sinks));
+            if (some) {
+                f32x16 s[2];
+                logits(lds + (t & 1) * TILE_B, s);
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) sees.hide(s[kb], kt, t, k0, k0 + 32 * kb + 4 * h, w.sinks, -INFINITY);
+                softmax(s);
+            }
+            tile_ready();
+            if (some) add_pv(lds + (2 + (t & 1)) * TILE_B, [&]() __attribute__((always_inline)) { fetch_v(t + 1); fetch_k(t + 2); });
+            else { fetch_v(t + 1); fetch_k(t + 2); }
+        }
+    };
+    masked_tiles(0, min(f0, ntiles));
+    const int first_after = max(f0, f1);
+    if (f0 < f1) {
+        const T* kp = Kh + (int64_t)kt.first_key(f0 + 2) * w.ks[2];
+        const T* vp = Vh + (int64_t)kt.first_key(f0 + 1) * w.vs[2];
+        const int64_t kstep = BN * w.ks[2], vstep = BN * w.vs[2];
+        int buf = f0 & 1;
+        for (int t = f0; t < f1; ++t) {
+            f32x16 s[2];
+            logits(lds + buf * TILE_B, s);
+            softmax(s);
+            tile_ready();
+            add_pv(lds + (2 + buf) * TILE_B, [&]() __attribute__((always_inline)) {
+                if (t + 2 < f1) {
+                    vfetch.fetch(vp, lds + (3 - buf) * TILE_B, true, [](int) { return true; });
+                    kfetch.fetch(kp, lds + buf * TILE_B, true, [](int) { return true; });
+                } else {
+                    fetch_v(t + 1);
+                    fetch_k(t + 2);
+                }
+            });
+            kp += kstep;
+            vp += vstep;
+            buf ^= 1;
         }
     }
+    masked_tiles(min(first_after, ntiles), ntiles);
 
     const float total = half_exchange_sum(l);
     if (qrow < w.Nq) {
@@ -338,7 +347,7 @@ int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
     if (nwg > 0x7fffffff) return fail(MYFA_E_UNSUPPORTED, "window attention: %lld query blocks", (long long)nwg);
     auto go = [&](auto kern) {
         launch_kernel(kern, dim3((unsigned)nwg), dim3(256), 0, s, static_cast<const T*>(q), static_cast<const T*>(k),
-                      static_cast<const T*>(v), static_cast<T*>(o), lse, w, nqblk, (int)nwg);
+                      static_cast<const T*>(v), static_cast<T*>(o), lse, w, nqblk);
     };
     if constexpr (sizeof(T) == 2) {
         if (w.d <= 64) go(window_attn_fwd16_kernel<T, 64>);
