@@ -65,7 +65,7 @@ int attn_bwd_mfma_static_ws(const void* q, const void* k, const void* v, const v
                             void* dq, void* dk, void* dv, int64_t heads, int64_t N, int64_t d,
                             float scale, int dtype, bool causal, hipStream_t s);
 int window_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const WindowShape& w, int dtype, hipStream_t s);
-int64_t window_attn_bwd_ws_bytes(const WindowShape& w);
+int64_t window_attn_bwd_ws_bytes(const WindowShape& w, int elem_size);
 int window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
                     void* dq, void* dk, void* dv, float* ws, const WindowShape& w, int dtype, hipStream_t s);
 int paged_append(const void* k, const void* v, const PagedCache& c, const AppendShape& a, hipStream_t s);
@@ -348,11 +348,11 @@ int myfa_window_attn_fwd(const void* q, const void* k, const void* v, void* o, f
     return window_attn_fwd(q, k, v, o, lse, w, dtype, static_cast<hipStream_t>(stream));
 }
 
-int64_t myfa_window_attn_bwd_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nk, int64_t d, int64_t window, int64_t sinks) {
+int64_t myfa_window_attn_bwd_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nk, int64_t d, int64_t window, int64_t sinks, int dtype) {
     WindowShape w;
     if (window_shape("window attention backward", w, nullptr, B, H, Hkv, Nq, Nk, d, window, sinks, 1.f) != MYFA_OK || d > 256) return 0;
     if (B == 0 || Nk == 0 || d == 0) return 0;
-    return window_attn_bwd_ws_bytes(w);
+    return window_attn_bwd_ws_bytes(w, elem_size(dtype));
 }
 
 int myfa_window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
@@ -371,7 +371,7 @@ int myfa_window_attn_bwd(const void* q, const void* k, const void* v, const void
     for (const void* p : {q, k, v, o, dout, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
         if (misaligned(p)) return fail(MYFA_E_INVALID, "%s: tensors must be 16-byte aligned", what);
     if (int rc = window_strides(what, w, q_strides, k_strides, v_strides, dtype)) return rc;
-    if (int rc = check_workspace(what, workspace, workspace_bytes, window_attn_bwd_ws_bytes(w))) return rc;
+    if (int rc = check_workspace(what, workspace, workspace_bytes, window_attn_bwd_ws_bytes(w, elem_size(dtype)))) return rc;
     return window_attn_bwd(q, k, v, o, lse, dout, dq, dk, dv, static_cast<float*>(workspace), w, dtype, static_cast<hipStream_t>(stream));
 }
 

@@ -147,7 +147,7 @@ std::vector<Tensor> window_bwd(const Tensor& dout, const Tensor& q, const Tensor
     const c10::DeviceGuard guard(q.device());
     const auto opt = q.options().memory_format(at::MemoryFormat::Contiguous);
     Tensor dq = at::empty({w.B, w.H, w.nq, w.d}, opt), dk = at::empty({w.B, w.G, w.nk, w.d}, opt), dv = at::empty({w.B, w.G, w.nk, w.d}, opt);
-    const int64_t bytes = myfa_window_attn_bwd_ws_bytes(w.B, w.H, w.G, w.nq, w.nk, w.d, w.window, w.sinks);
+    const int64_t bytes = myfa_window_attn_bwd_ws_bytes(w.B, w.H, w.G, w.nq, w.nk, w.d, w.window, w.sinks, tag(q));
     Tensor ws = at::empty({bytes}, opt.dtype(at::kByte));
     check(myfa_window_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr<float>(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(),
                                dv.data_ptr(), ints(lens), w.B, w.H, w.G, w.nq, w.nk, w.d, qs.s, ks.s, vs.s, w.window, w.sinks, (float)scale, tag(q),

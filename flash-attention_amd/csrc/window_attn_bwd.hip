@@ -255,7 +255,7 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
         f32x16 s[2], dp[2];
         typename M::vec8 sb[4];
         auto pds = [&](int kb, int i) __attribute__((always_inline)) {
-            s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], sl2, -lse2)) * (dp[kb][i] + ndelta);
+            s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], sl2, -lse2)) * dp[kb][i];
         };
         auto finish = [&](int kb) __attribute__((always_inline)) {
             if (edge) sees.hide(s[kb], kt, t, k0, k0 + 32 * kb + 4 * h, w.sinks, 0.f);
@@ -266,7 +266,7 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) { s[kb][i] = 0.f; dp[kb][i] = 0.f; }
+                for (int i = 0; i < 16; ++i) { s[kb][i] = 0.f; dp[kb][i] = ndelta; }
             auto block = [&](auto kb_, auto&& after) __attribute__((always_inline)) {
                 constexpr int kb = decltype(kb_)::value;
                 mma_stream<2 * KS, FW>([&](auto ic) __attribute__((always_inline)) {
@@ -331,6 +331,111 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
     }
 }
 
+// Few rows (see window_attn_common.h): 32 rows a workgroup, wave x takes tiles x, x + 4, ... of 32 keys.
+template <typename T, int D>
+__global__ void __launch_bounds__(256, 1)
+window_bwd_dq_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
+                         const T* __restrict__ dOg, const T* __restrict__ Og, const float* __restrict__ LSEg, float* __restrict__ st, T* __restrict__ dQg,
+                         WindowShape w, int nqp, int64_t rows, int nqblk) {
+    using R = TileReader<T, D>;
+    constexpr int BN = 32, NBUF = few_bufs<T, D>(), TILE_B = BN * R::RB, WAVE_B = few_wave_bytes<T, D>();
+    static_assert(WAVE_B >= 32 * D * 4, "a wave's sums fit its tiles");
+    __shared__ __attribute__((aligned(1024))) char lds[4 * WAVE_B];
+
+    const Ranked at_ = ranked(blockIdx.x, w.B * w.H);
+    const int bh = at_.head, q0 = (nqblk - 1 - at_.rank) * 32;
+    const int b = bh / w.H, head = bh - b * w.H, kvh = head / (w.H / w.Hkv);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5;
+    const KeyTiles<BN> kt(w, b, q0, 32);
+    const int ntiles = kt.ntiles;
+    const int qrow = q0 + r, p_own = qrow + kt.shift;
+    const bool live = qrow < w.Nq && p_own < kt.len;
+    const RowSees sees{p_own - w.window + 1, live ? p_own : -1};
+
+    const T* Kh = Kg + b * w.ks[0] + kvh * w.ks[1];
+    const T* Vh = Vg + b * w.vs[0] + kvh * w.vs[1];
+    const R rd(lane);
+    const TileFetch<T, D, BN, 64> kfetch(lane, w.ks[2], w.d), vfetch(lane, w.vs[2], w.d);
+    char* own = lds + wave * WAVE_B;
+    auto fetch = [&](int t, char* to) __attribute__((always_inline)) {
+        if (t >= ntiles) return;
+        const int k0 = kt.first_key(t);
+        const bool all = kt.all(k0, w.sinks);
+        auto keep = [&](int row) { return kt.one(k0 + row, w.sinks); };
+        kfetch.fetch(Kh + (int64_t)k0 * w.ks[2], to, all, keep);
+        vfetch.fetch(Vh + (int64_t)k0 * w.vs[2], to + TILE_B, all, keep);
+    };
+#pragma unroll
+    for (int i = 0; i < NBUF; ++i) fetch(wave + 4 * i, own + i * 2 * TILE_B);
+
+    typename R::frag qf[R::KS], of[R::KS];
+    const int row = min(qrow, w.Nq - 1);
+    {
+        constexpr int EPC = 16 / (int)sizeof(T);
+        const T* qp = Qg + b * w.qs[0] + head * w.qs[1] + (int64_t)row * w.qs[2];
+        const T* op = dOg + ((int64_t)bh * w.Nq + row) * w.d;
+#pragma unroll
+        for (int ks = 0; ks < R::KS; ++ks) {
+            const int c = (2 * ks + h) * EPC;
+            qf[ks] = typename R::frag{};
+            of[ks] = typename R::frag{};
+            if (c < w.d) {
+                qf[ks] = *reinterpret_cast<const typename R::frag*>(qp + c);
+                of[ks] = *reinterpret_cast<const typename R::frag*>(op + c);
+            }
+        }
+    }
+    const int64_t orow = (int64_t)bh * w.Nq + row;
+    const RowStat stat = row_stat<T>(of, Og + orow * w.d, LSEg + orow, live, w.d, h, st, rows, (int64_t)bh * nqp + qrow, wave == 0 && qrow < nqp);
+    const float sl2 = w.scale * kLog2eW;
+
+    f32x16 dq[R::DB];
+#pragma unroll
+    for (int db = 0; db < R::DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dq[db][i] = 0.f;
+
+    int buf = 0;
+    for (int t = wave; t < ntiles; t += 4) {
+        const int k0 = kt.first_key(t);
+        const char* Kb = own + buf * 2 * TILE_B;
+        wave_fetched();
+        f32x16 s, dp;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = stat.ndelta; }
+#pragma unroll
+        for (int ks = 0; ks < R::KS; ++ks) s = mma_chunk<T>(rd.row(Kb, 0, ks), qf[ks], s);
+#pragma unroll
+        for (int ks = 0; ks < R::KS; ++ks) dp = mma_chunk<T>(rd.row(Kb + TILE_B, 0, ks), of[ks], dp);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sl2, -stat.lse2)) * dp[i];
+        if (!(k0 + BN - 1 <= kt.pa && kt.pz == kt.pa + 32 && (k0 >= kt.pa + 32 - w.window || k0 + BN <= w.sinks)))
+            sees.hide(s, kt, t, k0, k0 + 4 * h, w.sinks, 0.f);
+        rd.add_transposed(Kb, 0, s, dq);
+        wave_read();
+        fetch(t + 4 * NBUF, own + buf * 2 * TILE_B);
+        buf = NBUF == 2 ? buf ^ 1 : 0;
+    }
+
+    put_sums(reinterpret_cast<float*>(own), dq, r, h);
+    __syncthreads();
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int e = tid; e < 32 * D / 4; e += 256) {
+        const int rw = e / (D / 4), col = (e - rw * (D / 4)) * 4;
+        if (q0 + rw >= w.Nq) break;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * WAVE_B) + sum_at<D>(rw, col));
+        const bool sees_any = q0 + rw + kt.shift < kt.len;
+        vec4 y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = sees_any ? (T)(sum[j] * w.scale) : (T)0.f;
+        if (col < w.d) *reinterpret_cast<vec4*>(dQg + ((int64_t)bh * w.Nq + q0 + rw) * w.d + col) = y;
+    }
+}
+
 // ---------------------------------------------------------------- dK, dV
 template <typename T, int D>
 __global__ void __launch_bounds__(256, D * sizeof(T) <= 128 ? 2 : 1)
@@ -365,6 +470,7 @@ window_bwd_dkv_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const 
     const int krow = k0 + 32 * wave + r;
     // positions that see the lane's key
     const int p_lo = krow, p_hi = krow >= w.Nk ? -1 : krow < w.sinks ? len - 1 : min(len - 1, krow + w.window - 1);
+    const bool seen = max(p_lo, shift) <= p_hi;      // a key that no query sees counts as zeros, whatever stands there
     const int key_a = k0 + 32 * wave, key_z = key_a + 31;                 // the wave's keys
 
     constexpr int EPC = 16 / (int)sizeof(T);
@@ -378,7 +484,7 @@ window_bwd_dkv_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const 
             const int c = (2 * ks + h) * EPC;
             kf[ks] = typename R::frag{};
             vf[ks] = typename R::frag{};
-            if (c < w.d) {
+            if (c < w.d && seen) {
                 kf[ks] = *reinterpret_cast<const typename R::frag*>(kp + c);
                 vf[ks] = *reinterpret_cast<const typename R::frag*>(vp + c);
             }
@@ -523,6 +629,7 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
 
     const int krow = k0 + 32 * wave + r;
     const int p_lo = krow, p_hi = krow >= w.Nk ? -1 : krow < w.sinks ? len - 1 : min(len - 1, krow + w.window - 1);
+    const bool seen = max(p_lo, shift) <= p_hi;      // a key that no query sees counts as zeros, whatever stands there
 
     s16x8 kf_[KS], vf_[KS];
     {
@@ -534,7 +641,7 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
             const int c = (2 * ks + h) * 8;
             kf_[ks] = s16x8{};
             vf_[ks] = s16x8{};
-            if (c < w.d) {
+            if (c < w.d && seen) {
                 kf_[ks] = *reinterpret_cast<const s16x8*>(kp + c);
                 vf_[ks] = *reinterpret_cast<const s16x8*>(vp + c);
             }
@@ -547,13 +654,17 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
 
     const R rd(lane);
     const F qfetch(tid, w.qs[2], w.d), ofetch(tid, w.d, w.d);
-    // where tile j (clamped to the last) of the flat list begins
-    struct At { const T *q, *o; const float* s; int p; };
-    auto at = [&](int j) __attribute__((always_inline)) {
-        j = min(j, j1 - 1);
-        const int g = j / nt, i0 = (tq0 + j - g * nt) * BQ, head = kvh * group + g;
-        const int64_t bh = (int64_t)b * w.H + head;
-        return At{Qg + b * w.qs[0] + head * w.qs[1] + (int64_t)i0 * w.qs[2], dOg + (bh * w.Nq + i0) * w.d, st + bh * nqp + i0, i0 + shift};
+    // A place in the flat list of tiles, head after head: tile x of head g, and where its rows begin.
+    struct At { const T *q, *o; const float* s; int p, x; };
+    const int64_t qstep = BQ * w.qs[2], ostep = (int64_t)BQ * w.d;
+    const int64_t qhead = w.qs[1] - (nt - 1) * qstep, ohead = (int64_t)w.Nq * w.d - (nt - 1) * ostep, shead = nqp - (nt - 1) * BQ;
+    auto next_of = [&](At& a) __attribute__((always_inline)) {
+        const bool wrap = a.x + 1 == nt;
+        a.q += wrap ? qhead : qstep;
+        a.o += wrap ? ohead : ostep;
+        a.s += wrap ? shead : (int64_t)BQ;
+        a.p = wrap ? tq0 * BQ + shift : a.p + BQ;
+        a.x = wrap ? 0 : a.x + 1;
     };
     // piece p of a tile's fetch: even p chunk set p / 2 of Q, odd p that of dO (p < 2 LPT), then the row statistics (wave 0).
     // Rows that see no key of the block read as zeros.
@@ -573,8 +684,7 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
         }
 #endif
     };
-    auto fetch_tile = [&](int j, int buf) __attribute__((always_inline)) {
-        const At a = at(j);
+    auto fetch_tile = [&](const At& a, int buf) __attribute__((always_inline)) {
         static_for<2 * LPT + 1>([&](auto ic) __attribute__((always_inline)) { fetch_piece(a, buf, ic); });
     };
 
@@ -589,15 +699,14 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
     constexpr int NSTEP = 8 * KS, FW = 8, PSTEP = FW / (2 * LPT);
     static_assert(PSTEP >= 1 && PSTEP * 2 * LPT == FW, "the tile's loads fill its last FW steps");
     int cur = 0, nxt = 1, fre = 2;
+    At ahead{};                                    // tile j + 2, or the last one
+    int pt = 0, left = 0;                          // the position tile j begins at; tiles behind `ahead`
 
-    auto tile = [&](int j, auto edge_) __attribute__((always_inline)) {
+    auto tile = [&](auto edge_) __attribute__((always_inline)) {
         constexpr bool EDGE = decltype(edge_)::value != 0;
         const char* Qb = lds + cur * TILE_B;
         const char* dOb = lds + (3 + cur) * TILE_B;
         const float* lse2b = stat + cur * 2 * BQ;
-        const int pt = (tq0 + j % nt) * BQ + shift;
-        const At next = at(j + 2);
-
         f32x16 s[2], dp[2];
         f32x4 l4[2][4];
         vec8 pb[4], sb[4];
@@ -609,8 +718,9 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
                 const f32x4 nd = *reinterpret_cast<const f32x4*>(lse2b + BQ + 32 * qb + 8 * g + 4 * h);
                 dp[qb][4 * g] = nd[0]; dp[qb][4 * g + 1] = nd[1]; dp[qb][4 * g + 2] = nd[2]; dp[qb][4 * g + 3] = nd[3];
             }
-        // element c = 32 qb + 8 (i >> 2) + (i & 3) of this lane is masked iff c > c_hi or c < c_lo
-        [[maybe_unused]] const int c_hi = p_hi - (pt + 4 * h), c_lo = p_lo - (pt + 4 * h);
+        // element c = 32 qb + 8 (i >> 2) + (i & 3) of this lane is seen iff c_lo <= c <= c_lo + c_span
+        [[maybe_unused]] const int c_lo = p_hi < p_lo ? 1 << 30 : p_lo - (pt + 4 * h);
+        [[maybe_unused]] const unsigned c_span = p_hi < p_lo ? 0u : (unsigned)(p_hi - p_lo);
 
         auto frag = [&](auto gc) __attribute__((always_inline)) -> s16x8 {
             constexpr int g = decltype(gc)::value;
@@ -645,11 +755,10 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
                 s[qb][e] = __builtin_fmaf(s[qb][e], sl2, -l4[qb][e >> 2][e & 3]);
             } else if constexpr (kind == 1) {
                 const float pe = __builtin_amdgcn_exp2f(s[qb][e]);
-                if constexpr (EDGE) s[qb][e] = (c > c_hi || c < c_lo) ? 0.f : pe;
+                if constexpr (EDGE) s[qb][e] = (unsigned)(c - c_lo) > c_span ? 0.f : pe;
                 else s[qb][e] = pe;
             } else if constexpr (kind == 2) {
-                if constexpr (EDGE) dp[qb][e] = (c > c_hi || c < c_lo) ? 0.f : s[qb][e] * dp[qb][e];   // (dP may be anything there)
-                else dp[qb][e] *= s[qb][e];
+                dp[qb][e] *= s[qb][e];
             } else if constexpr (kind == 3) {
                 pb[2 * qb + (e >> 2)][(2 * e) & 7] = (T)s[qb][2 * e];
                 pb[2 * qb + (e >> 2)][((2 * e) & 7) + 1] = (T)s[qb][2 * e + 1];
@@ -662,8 +771,8 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
             constexpr int g = decltype(gc)::value;
             // this wave's pieces of tile j + 1, requested a tile ago, are confirmed before those of j + 2 go out
             if constexpr (g == NSTEP - FW) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if constexpr (g >= NSTEP - FW && (g - (NSTEP - FW)) % PSTEP == 0) fetch_piece(next, fre, IC<(g - (NSTEP - FW)) / PSTEP>{});
-            if constexpr (g == NSTEP - 1) fetch_piece(next, fre, IC<2 * LPT>{});
+            if constexpr (g >= NSTEP - FW && (g - (NSTEP - FW)) % PSTEP == 0) fetch_piece(ahead, fre, IC<(g - (NSTEP - FW)) / PSTEP>{});
+            if constexpr (g == NSTEP - 1) fetch_piece(ahead, fre, IC<2 * LPT>{});
             constexpr int o0 = Plan::plan.start[g], o1 = Plan::plan.start[g + 1];
             static_for<o1 - o0>([&](auto oc) __attribute__((always_inline)) { vop(IC<o0 + decltype(oc)::value>{}); });
         });
@@ -676,16 +785,36 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
     };
 
     if (j0 < j1) {
-        fetch_tile(j0, 0);
-        fetch_tile(j0 + 1, 1);
+        {
+            const int g = j0 / nt, x = j0 - g * nt, i0 = (tq0 + x) * BQ, head = kvh * group + g;
+            const int64_t bh = (int64_t)b * w.H + head;
+            ahead = At{Qg + b * w.qs[0] + head * w.qs[1] + (int64_t)i0 * w.qs[2], dOg + (bh * w.Nq + i0) * w.d, st + bh * nqp + i0, i0 + shift, x};
+        }
+        int x = ahead.x;
+        pt = ahead.p;
+        left = j1 - 1 - j0;
+        auto step = [&]() __attribute__((always_inline)) { if (left > 0) { next_of(ahead); --left; } };
+        fetch_tile(ahead, 0);
+        step();
+        fetch_tile(ahead, 1);
+        step();
         tile_ready();
-        for (int j = j0; j < j1;) {
+        auto run = [&](int n, auto edge_) __attribute__((always_inline)) {
+            for (; n > 0; --n) {
+                tile(edge_);
+                step();
+                pt += BQ;
+            }
+        };
+        for (int todo = j1 - j0; todo > 0;) {
             // a head's tiles: masked ones, whole ones, masked ones
-            const int g = j / nt, x = j - g * nt;
             const bool edge = x < m0 || x >= m1;
-            const int end = min(j1, g * nt + (x < m0 ? min(m0, nt) : edge ? nt : m1));
-            if (edge) for (; j < end; ++j) tile(j, IC<1>{});
-            else for (; j < end; ++j) tile(j, IC<0>{});
+            const int end = x < m0 ? min(m0, nt) : edge ? nt : m1, n = min(todo, end - x);
+            if (edge) run(n, IC<1>{});
+            else run(n, IC<0>{});
+            todo -= n;
+            x += n;
+            if (x == nt) { x = 0; pt = tq0 * BQ + shift; }
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // nothing in flight into an LDS that is given up
     }
@@ -715,25 +844,167 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
         }
 }
 
+// Few rows (see window_attn_common.h): 32 keys a workgroup, wave x takes every fourth of the query tiles of 32.
+template <typename T, int D>
+__global__ void __launch_bounds__(256, 1)
+window_bwd_dkv_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
+                          const T* __restrict__ dOg, const float* __restrict__ st, T* __restrict__ dKg, T* __restrict__ dVg,
+                          float* __restrict__ parts, WindowShape w, int nqp, int64_t rows, int nsb, int ns) {
+    using R = TileReader<T, D>;
+    constexpr int BQ = 32, NBUF = few_bufs<T, D>(), TILE_B = BQ * R::RB, WAVE_B = few_wave_bytes<T, D>();
+    constexpr int ODB = R::DB < 4 ? R::DB : 4, NC = R::DB / ODB, C = 32 * ODB;
+    static_assert(WAVE_B >= 2 * 32 * C * 4, "a wave's sums fit its tiles");
+    __shared__ __attribute__((aligned(1024))) char lds[4 * WAVE_B];
+    __shared__ __attribute__((aligned(16))) float stats[4][NBUF][2][32];
+
+    const int lid = blockIdx.x / NC, col0 = ((int)blockIdx.x - lid * NC) * C;
+    const Ranked at_ = ranked(lid, w.B * w.Hkv);
+    const int bg = at_.head, unit = at_.rank;
+    const bool split = unit < nsb * ns;
+    const int kblk = split ? unit / ns : unit - nsb * ns + nsb, part = split ? unit - kblk * ns : 0, nparts = split ? ns : 1;
+    const int b = bg / w.Hkv, kvh = bg - b * w.Hkv, group = w.H / w.Hkv;
+    const int k0 = kblk * 32;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5;
+    const int len = w.lens ? min(max(w.lens[b], 0), w.Nk) : w.Nk;
+    const int shift = w.Nk - w.Nq;
+    const int pa = max(k0, shift), pz = k0 < w.sinks ? len : min(len, k0 + 31 + w.window);
+    const int tq0 = (pa - shift) / BQ, nt = pz > pa ? (pz - shift + BQ - 1) / BQ - tq0 : 0;
+    const int total = nt * group;
+    const int j0 = (int)((int64_t)total * part / nparts), j1 = (int)((int64_t)total * (part + 1) / nparts);
+
+    const int krow = k0 + r;
+    const int p_lo = krow, p_hi = krow >= w.Nk ? -1 : krow < w.sinks ? len - 1 : min(len - 1, krow + w.window - 1);
+    const bool seen = max(p_lo, shift) <= p_hi;      // a key that no query sees counts as zeros, whatever stands there
+
+    const R rd(lane);
+    const TileFetch<T, D, BQ, 64> qfetch(lane, w.qs[2], w.d), ofetch(lane, w.d, w.d);
+    char* own = lds + wave * WAVE_B;
+    auto fetch = [&](int j, int buf) __attribute__((always_inline)) {
+        if (j >= j1) return;
+        const int g = j / nt, i0 = (tq0 + j - g * nt) * BQ;
+        const int head = kvh * group + g;
+        const int64_t bh = (int64_t)b * w.H + head;
+        char* to = own + buf * 2 * TILE_B;
+        const bool all = i0 + shift >= pa && i0 + BQ + shift <= pz;
+        auto keep = [&](int row) { const int p = i0 + row + shift; return (p >= pa) & (p < pz); };
+        qfetch.fetch(Qg + b * w.qs[0] + head * w.qs[1] + (int64_t)i0 * w.qs[2], to, all, keep);
+        ofetch.fetch(dOg + (bh * w.Nq + i0) * w.d, to + TILE_B, all, keep);
+#if defined(__HIP_DEVICE_COMPILE__)
+        if (lane < BQ) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(st + x * rows + bh * nqp + i0), 0, BQ * 4, 0x00020000);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)&stats[wave][buf][x][0], 4, lane * 4, 0, 0, 0);
+            }
+        }
+#endif
+    };
+#pragma unroll
+    for (int i = 0; i < NBUF; ++i) fetch(j0 + wave + 4 * i, i);
+
+    constexpr int EPC = 16 / (int)sizeof(T);
+    typename R::frag kf[R::KS], vf[R::KS];
+    {
+        const int row = min(krow, w.Nk - 1);
+        const T* kp = Kg + b * w.ks[0] + kvh * w.ks[1] + (int64_t)row * w.ks[2];
+        const T* vp = Vg + b * w.vs[0] + kvh * w.vs[1] + (int64_t)row * w.vs[2];
+#pragma unroll
+        for (int ks = 0; ks < R::KS; ++ks) {
+            const int c = (2 * ks + h) * EPC;
+            kf[ks] = typename R::frag{};
+            vf[ks] = typename R::frag{};
+            if (c < w.d && seen) {
+                kf[ks] = *reinterpret_cast<const typename R::frag*>(kp + c);
+                vf[ks] = *reinterpret_cast<const typename R::frag*>(vp + c);
+            }
+        }
+    }
+    const float sl2 = w.scale * kLog2eW;
+    f32x16 dk[ODB], dv[ODB];
+#pragma unroll
+    for (int db = 0; db < ODB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { dk[db][i] = 0.f; dv[db][i] = 0.f; }
+
+    int buf = 0;
+    for (int j = j0 + wave; j < j1; j += 4) {
+        const int g = j / nt, pt = (tq0 + j - g * nt) * BQ + shift;
+        const char* Qb = own + buf * 2 * TILE_B;
+        const char* Ob = Qb + TILE_B;
+        wave_fetched();
+        f32x16 s, dp;
+        f32x4 l4[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            l4[q] = *reinterpret_cast<const f32x4*>(&stats[wave][buf][0][8 * q + 4 * h]);
+            const f32x4 nd = *reinterpret_cast<const f32x4*>(&stats[wave][buf][1][8 * q + 4 * h]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { s[4 * q + e] = 0.f; dp[4 * q + e] = nd[e]; }
+        }
+#pragma unroll
+        for (int ks = 0; ks < R::KS; ++ks) s = mma_chunk<T>(rd.row(Qb, 0, ks), kf[ks], s);
+#pragma unroll
+        for (int ks = 0; ks < R::KS; ++ks) dp = mma_chunk<T>(rd.row(Ob, 0, ks), vf[ks], dp);
+        const bool edge = !(pt >= k0 + 31 && pt + BQ <= len && k0 + 31 < w.Nk && (k0 + 31 < w.sinks || pt + BQ - 1 < k0 + w.window));
+        const int c_lo = p_hi < p_lo ? 1 << 30 : p_lo - (pt + 4 * h);
+        const unsigned c_span = p_hi < p_lo ? 0u : (unsigned)(p_hi - p_lo);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sl2, -l4[i >> 2][i & 3]));
+            if (edge && (unsigned)(8 * (i >> 2) + (i & 3) - c_lo) > c_span) s[i] = 0.f;
+            dp[i] *= s[i];
+        }
+        rd.add_transposed(Ob + R::COLB * (col0 / 32), 0, s, dv);
+        rd.add_transposed(Qb + R::COLB * (col0 / 32), 0, dp, dk);
+        wave_read();
+        fetch(j + 4 * NBUF, buf);
+        buf = NBUF == 2 ? buf ^ 1 : 0;
+    }
+
+    put_sums(reinterpret_cast<float*>(own), dk, r, h);
+    put_sums(reinterpret_cast<float*>(own) + 32 * C, dv, r, h);
+    __syncthreads();
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int e = tid; e < 2 * 32 * C / 4; e += 256) {
+        const int which = e / (32 * C / 4), rw = (e / (C / 4)) & 31, col = (e & (C / 4 - 1)) * 4, c = col0 + col;
+        if (k0 + rw >= w.Nk || c >= w.d) continue;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * WAVE_B) + which * 32 * C + sum_at<C>(rw, col));
+        if (!which) sum *= w.scale;
+        if (split && ns > 1) {
+            *reinterpret_cast<f32x4*>(parts + ((((int64_t)(bg * nsb + kblk) * ns + part) * 2 + which) * 32 + rw) * w.d + c) = sum;
+        } else {
+            vec4 y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = (T)sum[j];
+            *reinterpret_cast<vec4*>((which ? dVg : dKg) + ((int64_t)bg * w.Nk + k0 + rw) * w.d + c) = y;
+        }
+    }
+}
+
 // ---------------------------------------------------------------- the split key blocks' parts, in order
 template <typename T>
 __global__ void __launch_bounds__(256)
-window_bwd_join_kernel(const float* __restrict__ parts, T* __restrict__ dKg, T* __restrict__ dVg, int Nk, int d, int nsb, int ns, int64_t n4) {
+window_bwd_join_kernel(const float* __restrict__ parts, T* __restrict__ dKg, T* __restrict__ dVg, int Nk, int d, int bk, int nsb, int ns, int64_t n4) {
     typedef T vec4 __attribute__((ext_vector_type(4)));
     const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (u >= n4) return;
     const int per_row = d / 4;
     const int c = (int)(u % per_row) * 4;
     int64_t x = u / per_row;
-    const int row = (int)(x % 128); x /= 128;
+    const int row = (int)(x % bk); x /= bk;
     const int which = (int)(x % 2); x /= 2;
     const int kblk = (int)(x % nsb);
     const int64_t bg = x / nsb;
-    const int krow = kblk * 128 + row;
+    const int krow = kblk * bk + row;
     if (krow >= Nk) return;
-    const float* p = parts + (((bg * nsb + kblk) * ns * 2 + which) * 128 + row) * (int64_t)d + c;
+    const float* p = parts + (((bg * nsb + kblk) * ns * 2 + which) * bk + row) * (int64_t)d + c;
     f32x4 sum = *reinterpret_cast<const f32x4*>(p);
-    for (int i = 1; i < ns; ++i) sum += *reinterpret_cast<const f32x4*>(p + (int64_t)i * 2 * 128 * d);
+    for (int i = 1; i < ns; ++i) sum += *reinterpret_cast<const f32x4*>(p + (int64_t)i * 2 * bk * d);
     vec4 y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = (T)sum[e];
@@ -741,64 +1012,77 @@ window_bwd_join_kernel(const float* __restrict__ parts, T* __restrict__ dKg, T* 
 }
 
 // ---------------------------------------------------------------- host
-struct BwdPlan { int nqp, nkblk, nsb, ns; int64_t rows, stat_floats, part_floats; };
+// The kernels for many rows: 16-bit elements up to 128 columns have their own.
+template <typename T, int D> struct Large {
+    static constexpr auto dq() { if constexpr (sizeof(T) == 2 && D <= 128) return window_bwd_dq16_kernel<T, D>; else return window_bwd_dq_kernel<T, D>; }
+    static constexpr auto dkv() { if constexpr (sizeof(T) == 2 && D <= 128) return window_bwd_dkv16_kernel<T, D>; else return window_bwd_dkv_kernel<T, D>; }
+};
+
+struct BwdPlan { bool few_q, few_k; int bk, nqp, nkblk, nsb, ns; int64_t rows, stat_floats, part_floats; };
 
 // How many workgroups share a key block with sinks: enough that none has more than about a plain block's
 // queries, at most 32 (the parts are written and read once more).
-BwdPlan bwd_plan(const WindowShape& w) {
+BwdPlan bwd_plan(const WindowShape& w, int elem_size) {
     BwdPlan p;
+    p.few_q = few_queries(w, elem_size);
+    p.few_k = few_keys(w, elem_size);
+    p.bk = p.few_k ? 32 : 128;
     p.nqp = (int)cdiv(w.Nq, kStatPad) * kStatPad;
     p.rows = (int64_t)w.B * w.H * p.nqp;
-    p.nkblk = (int)cdiv(w.Nk, 128);
-    const bool uneven = w.sinks > 0 && w.window + 128 < w.Nk;
-    p.nsb = uneven ? (int)cdiv(w.sinks, 128) : 0;
-    const int64_t each = cdiv(w.Nk, (int64_t)w.window + 128);
+    p.nkblk = (int)cdiv(w.Nk, p.bk);
+    const bool uneven = w.sinks > 0 && w.window + p.bk < w.Nk;
+    p.nsb = uneven ? (int)cdiv(w.sinks, p.bk) : 0;
+    const int64_t each = cdiv(w.Nk, (int64_t)w.window + p.bk);
     p.ns = p.nsb > 0 ? (int)(each < 32 ? each : 32) : 1;
     p.stat_floats = 2 * p.rows;
-    p.part_floats = p.ns > 1 ? (int64_t)w.B * w.Hkv * p.nsb * p.ns * 2 * 128 * w.d : 0;
+    p.part_floats = p.ns > 1 ? (int64_t)w.B * w.Hkv * p.nsb * p.ns * 2 * p.bk * w.d : 0;
     return p;
 }
 
 template <typename T>
 int launch_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
                void* dq, void* dk, void* dv, float* ws, const WindowShape& w, hipStream_t s) {
-    const BwdPlan p = bwd_plan(w);
+    const BwdPlan p = bwd_plan(w, (int)sizeof(T));
     float* st = ws;
     float* parts = ws + p.stat_floats;
-    const int nqblk = (int)cdiv(w.Nq, 128);
+    const int nqblk = (int)cdiv(w.Nq, p.few_q ? 32 : 128);
     const int64_t nq = (int64_t)w.B * w.H * nqblk, nkv = (int64_t)w.B * w.Hkv * (p.nsb * (int64_t)p.ns + p.nkblk - p.nsb) * (w.d > 128 ? 2 : 1);
     if (nq > 0x7fffffff || nkv > 0x7fffffff)
         return fail(MYFA_E_UNSUPPORTED, "window attention backward: too many blocks");
-    auto go = [&](auto kdq, auto kdkv) {
-        // (dQ first: it leaves the row statistics that dK, dV reads)
+    auto go_q = [&](auto kern) {
         if (nq > 0)
-            launch_kernel(kdq, dim3((unsigned)nq), dim3(256), 0, s, static_cast<const T*>(q), static_cast<const T*>(k),
+            launch_kernel(kern, dim3((unsigned)nq), dim3(256), 0, s, static_cast<const T*>(q), static_cast<const T*>(k),
                           static_cast<const T*>(v), static_cast<const T*>(dout), static_cast<const T*>(o), lse, st, static_cast<T*>(dq),
                           w, p.nqp, p.rows, nqblk);
-        launch_kernel(kdkv, dim3((unsigned)nkv), dim3(256), 0, s, static_cast<const T*>(q), static_cast<const T*>(k),
+    };
+    auto go_kv = [&](auto kern) {
+        launch_kernel(kern, dim3((unsigned)nkv), dim3(256), 0, s, static_cast<const T*>(q), static_cast<const T*>(k),
                       static_cast<const T*>(v), static_cast<const T*>(dout), st, static_cast<T*>(dk), static_cast<T*>(dv), parts,
                       w, p.nqp, p.rows, p.nsb, p.ns);
     };
-    if constexpr (sizeof(T) == 2) {
-        if (w.d <= 64) go(window_bwd_dq16_kernel<T, 64>, window_bwd_dkv16_kernel<T, 64>);
-        else if (w.d <= 128) go(window_bwd_dq16_kernel<T, 128>, window_bwd_dkv16_kernel<T, 128>);
-        else go(window_bwd_dq_kernel<T, 256>, window_bwd_dkv_kernel<T, 256>);
-    } else {
-        if (w.d <= 64) go(window_bwd_dq_kernel<T, 64>, window_bwd_dkv_kernel<T, 64>);
-        else go(window_bwd_dq_kernel<T, 128>, window_bwd_dkv_kernel<T, 128>);
+    // (dQ first: it leaves the row statistics that dK, dV reads)
+    if (w.d <= 64) {
+        go_q(p.few_q ? window_bwd_dq_few_kernel<T, 64> : Large<T, 64>::dq());
+        go_kv(p.few_k ? window_bwd_dkv_few_kernel<T, 64> : Large<T, 64>::dkv());
+    } else if (w.d <= 128) {
+        go_q(p.few_q ? window_bwd_dq_few_kernel<T, 128> : Large<T, 128>::dq());
+        go_kv(p.few_k ? window_bwd_dkv_few_kernel<T, 128> : Large<T, 128>::dkv());
+    } else if constexpr (sizeof(T) == 2) {
+        go_q(p.few_q ? window_bwd_dq_few_kernel<T, 256> : Large<T, 256>::dq());
+        go_kv(p.few_k ? window_bwd_dkv_few_kernel<T, 256> : Large<T, 256>::dkv());
     }
     if (p.ns > 1) {
-        const int64_t n4 = (int64_t)w.B * w.Hkv * p.nsb * 2 * 128 * (w.d / 4);
+        const int64_t n4 = (int64_t)w.B * w.Hkv * p.nsb * 2 * p.bk * (w.d / 4);
         launch_kernel(window_bwd_join_kernel<T>, dim3((unsigned)cdiv(n4, 256)), dim3(256), 0, s, parts, static_cast<T*>(dk),
-                      static_cast<T*>(dv), w.Nk, w.d, p.nsb, p.ns, n4);
+                      static_cast<T*>(dv), w.Nk, w.d, p.bk, p.nsb, p.ns, n4);
     }
     return check_launch("window attention backward");
 }
 
 }  // namespace
 
-int64_t window_attn_bwd_ws_bytes(const WindowShape& w) {
-    const BwdPlan p = bwd_plan(w);
+int64_t window_attn_bwd_ws_bytes(const WindowShape& w, int elem_size) {
+    const BwdPlan p = bwd_plan(w, elem_size);
     return (p.stat_floats + p.part_floats) * 4;
 }
 

@@ -340,9 +340,135 @@ window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
     }
 }
 
+// Few rows (see window_attn_common.h): 32 rows a workgroup, wave x takes tiles x, x + 4, ... of 32 keys.
+template <typename T, int D>
+__global__ void __launch_bounds__(256, D * sizeof(T) <= 128 ? 2 : 1)
+window_attn_fwd_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
+                           T* __restrict__ Og, float* __restrict__ LSEg, WindowShape w, int nqblk) {
+    using R = TileReader<T, D>;
+    constexpr int BN = 32, NBUF = few_bufs<T, D>(), TILE_B = BN * R::RB, WAVE_B = few_wave_bytes<T, D>();
+    static_assert(WAVE_B >= 32 * D * 4, "a wave's sums fit its tiles");
+    __shared__ __attribute__((aligned(1024))) char lds[4 * WAVE_B];
+    __shared__ float ml[4][2][32];
+
+    const Ranked at_ = ranked(blockIdx.x, w.B * w.H);
+    const int bh = at_.head, q0 = (nqblk - 1 - at_.rank) * 32;
+    const int b = bh / w.H, head = bh - b * w.H, kvh = head / (w.H / w.Hkv);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r = lane & 31, h = lane >> 5;
+    const KeyTiles<BN> kt(w, b, q0, 32);
+    const int ntiles = kt.ntiles;
+    const int qrow = q0 + r, p_own = qrow + kt.shift;
+    const bool live = qrow < w.Nq && p_own < kt.len;
+    const RowSees sees{p_own - w.window + 1, live ? p_own : -1};
+
+    const T* Kh = Kg + b * w.ks[0] + kvh * w.ks[1];
+    const T* Vh = Vg + b * w.vs[0] + kvh * w.vs[1];
+    const R rd(lane);
+    const TileFetch<T, D, BN, 64> kfetch(lane, w.ks[2], w.d), vfetch(lane, w.vs[2], w.d);
+    char* own = lds + wave * WAVE_B;
+    auto fetch = [&](int t, char* to) __attribute__((always_inline)) {
+        if (t >= ntiles) return;
+        const int k0 = kt.first_key(t);
+        const bool all = kt.all(k0, w.sinks);
+        auto keep = [&](int row) { return kt.one(k0 + row, w.sinks); };
+        kfetch.fetch(Kh + (int64_t)k0 * w.ks[2], to, all, keep);
+        vfetch.fetch(Vh + (int64_t)k0 * w.vs[2], to + TILE_B, all, keep);
+    };
+#pragma unroll
+    for (int i = 0; i < NBUF; ++i) fetch(wave + 4 * i, own + i * 2 * TILE_B);
+
+    typename R::frag qf[R::KS];
+    {
+        const T* qp = Qg + b * w.qs[0] + head * w.qs[1] + (int64_t)min(qrow, w.Nq - 1) * w.qs[2];
+        constexpr int EPC = 16 / (int)sizeof(T);
+#pragma unroll
+        for (int ks = 0; ks < R::KS; ++ks) {
+            const int c = (2 * ks + h) * EPC;
+            qf[ks] = typename R::frag{};
+            if (c < w.d) qf[ks] = *reinterpret_cast<const typename R::frag*>(qp + c);
+        }
+    }
+    f32x16 o[R::DB];
+#pragma unroll
+    for (int db = 0; db < R::DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const float sl2 = w.scale * kLog2eW;
+
+    int buf = 0;
+    for (int t = wave; t < ntiles; t += 4) {
+        const int k0 = kt.first_key(t);
+        const char* Kb = own + buf * 2 * TILE_B;
+        wave_fetched();
+        f32x16 s;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < R::KS; ++ks) s = mma_chunk<T>(rd.row(Kb, 0, ks), qf[ks], s);
+        if (!(k0 + BN - 1 <= kt.pa && kt.pz == kt.pa + 32 && (k0 >= kt.pa + 32 - w.window || k0 + BN <= w.sinks)))
+            sees.hide(s, kt, t, k0, k0 + 4 * h, w.sinks, -INFINITY);
+        float tmax = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) tmax = fmaxf(tmax, s[i]);
+        const float m_new = fmaxf(m, half_exchange_max(tmax) * sl2);
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = __builtin_amdgcn_exp2f(m - ref);
+        m = m_new;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], sl2, -ref));
+            sum += s[i];
+        }
+        l = l * alpha + sum;
+#pragma unroll
+        for (int db = 0; db < R::DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
+        rd.add_transposed(Kb + TILE_B, 0, s, o);
+        wave_read();
+        fetch(t + 4 * NBUF, own + buf * 2 * TILE_B);
+        buf = NBUF == 2 ? buf ^ 1 : 0;
+    }
+
+    l = half_exchange_sum(l);
+    if (h == 0) { ml[wave][0][r] = m; ml[wave][1][r] = l; }
+    put_sums(reinterpret_cast<float*>(own), o, r, h);
+    __syncthreads();
+    typedef T vec4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int e = tid; e < 32 * D / 4; e += 256) {
+        const int row = e / (D / 4), col = (e - row * (D / 4)) * 4;
+        if (q0 + row >= w.Nq) break;
+        const bool sees_any = q0 + row + kt.shift < kt.len;
+        float top = ml[0][0][row];
+#pragma unroll
+        for (int x = 1; x < 4; ++x) top = fmaxf(top, ml[x][0][row]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float total = 0.f;
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const float f = __builtin_amdgcn_exp2f(ml[x][0][row] - ref);
+            total += f * ml[x][1][row];
+            sum += f * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * WAVE_B) + sum_at<D>(row, col));
+        }
+        const float inv = 1.f / total;
+        vec4 y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = sees_any ? (T)(sum[j] * inv) : (T)0.f;
+        const int64_t at = (int64_t)bh * w.Nq + q0 + row;
+        if (col < w.d) *reinterpret_cast<vec4*>(Og + at * w.d + col) = y;
+        if (col == 0 && LSEg != nullptr) LSEg[at] = sees_any ? (top + __builtin_amdgcn_logf(total)) * kLn2W : -INFINITY;
+    }
+}
+
 template <typename T>
 int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const WindowShape& w, hipStream_t s) {
-    const int nqblk = (int)cdiv(w.Nq, 128);
+    const bool few = few_queries(w, (int)sizeof(T));
+    const int nqblk = (int)cdiv(w.Nq, few ? 32 : 128);
     const int64_t nwg = (int64_t)w.B * w.H * nqblk;
     if (nwg > 0x7fffffff) return fail(MYFA_E_UNSUPPORTED, "window attention: %lld query blocks", (long long)nwg);
     auto go = [&](auto kern) {
@@ -350,12 +476,12 @@ int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse,
                       static_cast<const T*>(v), static_cast<T*>(o), lse, w, nqblk);
     };
     if constexpr (sizeof(T) == 2) {
-        if (w.d <= 64) go(window_attn_fwd16_kernel<T, 64>);
-        else if (w.d <= 128) go(window_attn_fwd16_kernel<T, 128>);
-        else go(window_attn_fwd_kernel<T, 256>);
+        if (w.d <= 64) few ? go(window_attn_fwd_few_kernel<T, 64>) : go(window_attn_fwd16_kernel<T, 64>);
+        else if (w.d <= 128) few ? go(window_attn_fwd_few_kernel<T, 128>) : go(window_attn_fwd16_kernel<T, 128>);
+        else few ? go(window_attn_fwd_few_kernel<T, 256>) : go(window_attn_fwd_kernel<T, 256>);
     } else {
-        if (w.d <= 64) go(window_attn_fwd_kernel<T, 64>);
-        else go(window_attn_fwd_kernel<T, 128>);
+        if (w.d <= 64) few ? go(window_attn_fwd_few_kernel<T, 64>) : go(window_attn_fwd_kernel<T, 64>);
+        else few ? go(window_attn_fwd_few_kernel<T, 128>) : go(window_attn_fwd_kernel<T, 128>);
     }
     return check_launch("window attention");
 }

@@ -92,7 +92,7 @@ def _load():
     lib.myfa_matmul_f32.restype = ci
     lib.myfa_window_attn_fwd.argtypes = [vp] * 6 + [i64] * 6 + [vp] * 3 + [i64, i64, f32, ci, vp]
     lib.myfa_window_attn_fwd.restype = ci
-    lib.myfa_window_attn_bwd_ws_bytes.argtypes = [i64] * 8
+    lib.myfa_window_attn_bwd_ws_bytes.argtypes = [i64] * 8 + [ci]
     lib.myfa_window_attn_bwd_ws_bytes.restype = i64
     lib.myfa_window_attn_bwd.argtypes = [vp] * 10 + [i64] * 6 + [vp] * 3 + [i64, i64, f32, ci, vp, i64, vp]
     lib.myfa_window_attn_bwd.restype = ci

@@ -308,7 +308,7 @@ int myfa_window_attn_fwd(const void* q, const void* k, const void* v, void* o, f
  * calls that may overlap need one each.  No atomics: the result depends on the inputs alone.
  */
 int64_t myfa_window_attn_bwd_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nk, int64_t d,
-                                      int64_t window, int64_t sinks);
+                                      int64_t window, int64_t sinks, int dtype);
 int myfa_window_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
                          void* dq, void* dk, void* dv, const int32_t* seq_lens,
                          int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nk, int64_t d,

@@ -69,7 +69,7 @@ def test_c_abi_refusals_of_window_attention():
 
     def bwd(ws, nbytes, p=16):
         return lib.myfa_window_attn_bwd(*([p] * 9), None, 1, 2, 1, 4, 8, 64, st, st, st, 4, 0, 1.0, bf16, ws, nbytes, None)
-    need = lib.myfa_window_attn_bwd_ws_bytes(1, 2, 1, 4, 8, 64, 4, 0)
+    need = lib.myfa_window_attn_bwd_ws_bytes(1, 2, 1, 4, 8, 64, 4, 0, bf16)
     assert need >= 2 * 2 * 4 * 4
     _error(bwd(16, need - 1), 1, "workspace")
     _error(bwd(None, need), 1, "workspace")

@@ -78,6 +78,46 @@ def test_long_sequence(mfa):
     _compare(mfa, 1, 2, 1, 2100, 2100, 128, 300, 4, None, BF16)
 
 
+MANY = [
+    # enough blocks for the kernels that take 128 rows a workgroup
+    (8, 16, 16, 200, 200, 64, 1000, 0, None),
+    (4, 48, 48, 130, 333, 128, 64, 4, [333, 200, 203, 0]),
+    (2, 48, 24, 300, 300, 80, 33, 1, [300, 77]),
+    (1, 60, 30, 513, 513, 128, 90, 5, None),
+    (1, 48, 24, 640, 640, 64, 100, 130, None),
+    (3, 36, 12, 257, 400, 128, 170, 3, [400, 399, 150]),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("case", MANY, ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+def test_many_rows(mfa, case, dtype):
+    _compare(mfa, *case, dtype)
+
+
+@pytest.mark.parametrize("case", [(4, 48, 48, 130, 333, 128, 64, 4, [333, 200, 203, 0]), (1, 96, 96, 700, 700, 32, 90, 5, None)],
+                         ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+def test_many_rows_float32(mfa, case):
+    _compare(mfa, *case, F32)
+
+
+def test_many_rows_wide_heads(mfa):
+    _compare(mfa, 2, 72, 72, 140, 140, 192, 50, 3, [140, 90], BF16)
+
+
+@pytest.mark.parametrize("fill", [float("nan"), float("inf")])
+def test_padding_of_many_rows_may_hold_anything(mfa, fill):
+    lens = [200, 137, 0, 64]
+    q, k, v, dout = _inputs(4, 32, 32, 200, 200, 64, BF16, 1)
+    want = ref.attention(q, k, v, _visible(4, 200, 200, 30, 2, lens), 0.125, BF16, dout)
+    for b, n in enumerate(lens):
+        for t in (q, k, v, dout):
+            t[b, :, n:] = fill
+    got = _run(mfa, *(t.cuda() for t in (q, k, v, dout)), 30, 2, 0.125, lens)
+    for name in got:
+        ref.check(name, got[name], want[name])
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_gradients_against_differences(mfa, dtype):
     """The gradients of the definition itself, against central differences of it: what the bounds are held to is the
