@@ -95,25 +95,33 @@ paged_decode_kernel(const T* __restrict__ Qg, PagedCache c, T* __restrict__ Og, 
     const int* row_table = c.table + (int64_t)b * c.width;
     char* vt = lds + wave * WAVE_B;
 
-    // K and V rows i and 16 + i of a tile, chunks 4 s + g.  Keys that are not seen are zeros (V) and masked
-    // below (K); a key whose page number is not of the pool is NaN, so that its sequence's result is.
-    u32x4 kr[2][KS], vr[2][KS];
-    auto load = [&](int t) __attribute__((always_inline)) {
+    // Where keys i and 16 + i of a tile stand: looked up one tile ahead of the loads that need it, so that a tile's
+    // time does not hold the table's latency and then the cache's.
+    int page[2], slot[2];                       // page -1: a key that is not seen
+    auto look_up = [&](int t) __attribute__((always_inline)) {
         const int k0 = (t < sn.n_sink ? t : t - sn.n_sink + sn.t_win) * kKeys;
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
             const int key = k0 + 16 * blk + i;
-            const bool see = (key < sn.len) & ((key >= sn.lo) | (key < w.sinks));
-            int page = 0, slot = 0;
-            if (see) {
+            page[blk] = -1;
+            if ((key < sn.len) & ((key >= sn.lo) | (key < w.sinks))) {
                 const int pi = (int)c.page.div((uint32_t)key);
-                slot = key - pi * (int)c.page.d;
-                page = row_table[pi];
+                slot[blk] = key - pi * (int)c.page.d;
+                const int at = row_table[pi];
+                page[blk] = at == -1 ? -2 : at;
             }
-            const bool ok = see & (page >= 0) & (page < c.num_pages);
-            const char* kp = c.k + page * c.kst[0] + kvh * c.kst[1] + slot * c.kst[2];
-            const char* vp = c.v + page * c.vst[0] + kvh * c.vst[1] + slot * c.vst[2];
-            const unsigned fill = see && !ok ? 0x7FFF7FFFu : 0u;      // a NaN in all three types
+        }
+    };
+    // K and V rows i and 16 + i of the tile looked up, chunks 4 s + g.  Keys that are not seen are zeros (V) and
+    // masked below (K); a key whose page number is not of the pool is NaN, so that its sequence's result is.
+    u32x4 kr[2][KS], vr[2][KS];
+    auto load = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+            const bool ok = (page[blk] >= 0) & (page[blk] < c.num_pages);
+            const char* kp = c.k + page[blk] * c.kst[0] + kvh * c.kst[1] + slot[blk] * c.kst[2];
+            const char* vp = c.v + page[blk] * c.vst[0] + kvh * c.vst[1] + slot[blk] * c.vst[2];
+            const unsigned fill = page[blk] != -1 && !ok ? 0x7FFF7FFFu : 0u;      // a NaN in all three types
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 const int at = (4 * s + g) * 16;
@@ -134,7 +142,8 @@ paged_decode_kernel(const T* __restrict__ Qg, PagedCache c, T* __restrict__ Og, 
     const int tq = (lane & 15) >> 2, tp = lane & 3;
 
     int t = t0 + wave;
-    if (t < t1) load(t);
+    if (t < t1) { look_up(t); load(); }
+    if (t + 4 < t1) look_up(t + 4);
     for (; t < t1; t += 4) {
         const int k0 = (t < sn.n_sink ? t : t - sn.n_sink + sn.t_win) * kKeys;
 #pragma unroll
@@ -151,7 +160,8 @@ paged_decode_kernel(const T* __restrict__ Qg, PagedCache c, T* __restrict__ Og, 
 #pragma unroll
             for (int s = 0; s < KS; ++s) sc[blk] = mma16_chunk<T>(__builtin_bit_cast(frag, kr[blk][s]), qf[s], sc[blk]);
         }
-        if (t + 4 < t1) load(t + 4);
+        if (t + 4 < t1) load();
+        if (t + 8 < t1) look_up(t + 8);
 
         // lane (i, g): head i, keys k0 + 16 blk + 4 g + r
         const bool edge = k0 + kKeys > sn.len || (k0 < sn.lo && k0 + kKeys > w.sinks);
@@ -260,41 +270,50 @@ paged_decode_kernel(const T* __restrict__ Qg, PagedCache c, T* __restrict__ Og, 
     }
 }
 
-// Maximum and sum of a head over its shares.
-struct TopSum { float top, total; };
-__device__ __forceinline__ TopSum join_ml(const float* ml, int ns) {
-    TopSum j{-INFINITY, 0.f};
-    for (int s = 0; s < ns; ++s) j.top = fmaxf(j.top, ml[2 * s]);
-    const float ref = j.top == -INFINITY ? 0.f : j.top;
-    for (int s = 0; s < ns; ++s) j.total += __builtin_amdgcn_exp2f(ml[2 * s] - ref) * ml[2 * s + 1];
+// Maximum and sum of a head over its ns shares; the lanes of a wave take them in turn and all get the result.
+struct TopSum { float top, ref, total; };
+__device__ __forceinline__ TopSum join_ml(const float* ml, int ns, int lane) {
+    TopSum j{-INFINITY, 0.f, 0.f};
+    for (int s = lane; s < ns; s += 64) j.top = fmaxf(j.top, ml[2 * s]);
+    j.top = wave_max(j.top);
+    j.ref = j.top == -INFINITY ? 0.f : j.top;
+    for (int s = lane; s < ns; s += 64) j.total += __builtin_amdgcn_exp2f(ml[2 * s] - j.ref) * ml[2 * s + 1];
+    j.total = wave_sum(j.total);
     return j;
 }
 
-// Workgroups [0, njoin): four query heads each, one per wave (none where every head had one share).  The
-// others: 1024 keys of one key/value head, four per thread.
+// Workgroups [0, njoin): one query head each (none where every head had one share); D / 4 threads take a share's
+// columns, the workgroup's groups of so many every share in turn, and their sums meet in LDS in order.  The others:
+// 1024 keys of one key/value head, four per thread.
 template <typename T>
 __global__ void __launch_bounds__(256)
 paged_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const float* __restrict__ scores,
                   T* __restrict__ Og, float* __restrict__ LSEg, float* __restrict__ weight_sum, DecodeShape w,
                   int cap, int ns, int D, int njoin, int nchunk, int64_t score_row) {
+    __shared__ __attribute__((aligned(16))) float lds[1024];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if ((int)blockIdx.x < njoin) {
-        const int64_t bh = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-        if (bh >= (int64_t)w.B * w.H) return;
-        const int lane = threadIdx.x & 63, len = w.lens[bh / w.H];
+        const int64_t bh = blockIdx.x;
+        const int len = w.lens[bh / w.H];
         const float* ml = part_ml + bh * ns * 2;
-        const TopSum j = join_ml(ml, ns);
-        const float ref = j.top == -INFINITY ? 0.f : j.top, inv = 1.f / j.total;
-        for (int col = 4 * lane; col < w.d; col += 256) {
-            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-            for (int s = 0; s < ns; ++s)
-                sum += __builtin_amdgcn_exp2f(ml[2 * s] - ref) * *reinterpret_cast<const f32x4*>(part_o + (bh * ns + s) * D + col);
+        const TopSum j = join_ml(ml, ns, lane);
+        const int tpg = D / 4, grp = tid / tpg, groups = 256 / tpg, col = 4 * (tid - grp * tpg);
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int s = grp; s < ns; s += groups)
+            sum += __builtin_amdgcn_exp2f(ml[2 * s] - j.ref) * *reinterpret_cast<const f32x4*>(part_o + (bh * ns + s) * D + col);
+        *reinterpret_cast<f32x4*>(lds + 4 * tid) = sum;
+        __syncthreads();
+        if (grp == 0 && col < w.d) {
+            for (int g = 1; g < groups; ++g) sum += *reinterpret_cast<const f32x4*>(lds + 4 * (tid + g * tpg));
+            const float inv = 1.f / j.total;
             typedef T vec4 __attribute__((ext_vector_type(4)));
             vec4 y;
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[r] = len > 0 ? (T)(sum[r] * inv) : (T)0.f;
             *reinterpret_cast<vec4*>(Og + bh * w.d + col) = y;
+            if (col == 0 && LSEg != nullptr) LSEg[bh] = len > 0 ? (j.top + __builtin_amdgcn_logf(j.total)) * kLn2P : -INFINITY;
         }
-        if (lane == 0 && LSEg != nullptr) LSEg[bh] = len > 0 ? (j.top + __builtin_amdgcn_logf(j.total)) * kLn2P : -INFINITY;
         return;
     }
     const int u = blockIdx.x - njoin;
@@ -302,24 +321,24 @@ paged_join_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
     const int b = bg / w.Hkv, kvh = bg - b * w.Hkv, group = w.H / w.Hkv;
     const Seen sn = seen_of(w.lens[b], cap, w.window, w.sinks);
     // chunks of the tiles that the first launch went through, as they follow each other there
-    const int vt = chunk * 32 + (threadIdx.x >> 3);
+    const int vt = chunk * 32 + (tid >> 3);
     if (chunk * 32 >= sn.ntiles) return;
-    __shared__ float lse2[64];
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    const int key = (vt < sn.n_sink ? vt : vt - sn.n_sink + sn.t_win) * kKeys + (threadIdx.x & 7) * 4;
+    const int key = (vt < sn.n_sink ? vt : vt - sn.n_sink + sn.t_win) * kKeys + (tid & 7) * 4;
     for (int h0 = 0; h0 < group; h0 += 64) {
-        __syncthreads();
         const int n = min(64, group - h0);
-        if ((int)threadIdx.x < n) {
-            const TopSum j = join_ml(part_ml + ((int64_t)b * w.H + kvh * group + h0 + threadIdx.x) * ns * 2, ns);
-            lse2[threadIdx.x] = j.top + __builtin_amdgcn_logf(j.total);
+        __syncthreads();
+        for (int x = wave; x < n; x += 4) {
+            const TopSum j = join_ml(part_ml + ((int64_t)b * w.H + kvh * group + h0 + x) * ns * 2, ns, lane);
+            if (lane == 0) lds[x] = j.top + __builtin_amdgcn_logf(j.total);
         }
         __syncthreads();
         if (vt < sn.ntiles)
+#pragma unroll 4
             for (int x = 0; x < n; ++x) {
                 const f32x4 s = *reinterpret_cast<const f32x4*>(scores + ((int64_t)b * w.H + kvh * group + h0 + x) * score_row + key);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum[e] += __builtin_amdgcn_exp2f(s[e] - lse2[x]);
+                for (int e = 0; e < 4; ++e) sum[e] += __builtin_amdgcn_exp2f(s[e] - lds[x]);
             }
     }
     if (vt < sn.ntiles) {
@@ -357,8 +376,11 @@ int pad_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 struct DecodePlan { int ns, D, qtiles; int64_t score_row, ml_floats, o_floats, score_floats; };
 
-// Shares per head: enough workgroups that the chip is full several times over (the lengths are on the device,
-// and sequences differ), as long as every wave of a share has two tiles of the longest possible sequence.
+// Shares per head: enough workgroups that the chip is full several times over (the lengths are on the device, and
+// sequences differ), as long as every wave of a share has two tiles of the longest possible sequence; one share where
+// its waves have four tiles or fewer, which saves the second launch.  Measured (us, workgroups aimed at 1024 / 2048 /
+// 4096 / 8192): 8 sequences up to 131072 keys 499 / 505 / 485 / 503, 64 up to 4096 171 / 157 / 153 / 157; tiles per
+// wave 1 / 2 / 4 / 8: one sequence of 1024 keys 12.3 / 12.7 / 17.1 / 23.2; at most 300 keys, split / not: 12.7 / 10.3.
 DecodePlan decode_plan(const DecodeShape& w, int64_t cap, bool weights) {
     DecodePlan p;
     p.D = pad_dim(w.d);
@@ -366,7 +388,7 @@ DecodePlan decode_plan(const DecodeShape& w, int64_t cap, bool weights) {
     const int64_t base = (int64_t)w.B * w.Hkv * p.qtiles;
     int64_t seen = cap;
     if ((int64_t)w.window + w.sinks < cap) seen = (int64_t)w.window + w.sinks;
-    const int64_t most = cdiv(cdiv(seen, kKeys), 8);
+    const int64_t tiles = cdiv(seen, kKeys), most = tiles <= 16 ? 1 : cdiv(tiles, 8);
     int64_t ns = cdiv(4096, base > 0 ? base : 1);
     if (ns > most) ns = most;
     if (ns > 128) ns = 128;
@@ -385,7 +407,7 @@ int launch_decode(const void* q, const PagedCache& c, void* o, float* lse, float
     const DecodePlan p = decode_plan(w, cap, weight_sum != nullptr);
     const int64_t nwg = (int64_t)w.B * w.Hkv * p.qtiles * p.ns;
     const int nchunk = weight_sum ? (int)cdiv(cdiv(cap, kKeys) + 1, 32) : 0;
-    const int64_t njoin = p.ns > 1 ? cdiv((int64_t)w.B * w.H, 4) : 0, nw = (int64_t)w.B * w.Hkv * nchunk;
+    const int64_t njoin = p.ns > 1 ? (int64_t)w.B * w.H : 0, nw = (int64_t)w.B * w.Hkv * nchunk;
     if (nwg > 0x7fffffff || njoin + nw > 0x7fffffff) return fail(MYFA_E_UNSUPPORTED, "paged attention: too many workgroups");
     float* ml = p.ml_floats ? ws + p.o_floats : nullptr;
     float* scores = weight_sum ? ws + p.o_floats + p.ml_floats : nullptr;

@@ -46,6 +46,9 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* waves, uint
     return x + before;
 }
 
+// PER > 0: a thread holds up to PER consecutive sums of the row in registers (rows of up to PER * 1024 keys); PER = 0: the
+// row is read again in every pass.
+template <int PER>
 __global__ void __launch_bounds__(kSelThreads)
 paged_evict_select_kernel(EvictShape e) {
     __shared__ uint32_t hist[kBins], waves[kSelWaves], found[2];
@@ -54,6 +57,18 @@ paged_evict_select_kernel(EvictShape e) {
     const float* sums = e.sums + (int64_t)bg * e.cap;
     float* new_sums = e.new_sums + (int64_t)bg * e.new_cap;
     int* kept = e.kept + (int64_t)bg * e.budget;
+
+    constexpr int HELD = PER > 0 ? PER : kPer;
+    const int per = PER > 0 ? (len + kSelThreads - 1) / kSelThreads : kPer;       // consecutive keys of a thread
+    float x[HELD];
+    auto read = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < HELD; ++j) {
+            const int i = i0 + tid * per + j;
+            x[j] = j < per && i < len ? sums[i] : 0.f;
+        }
+    };
+    if constexpr (PER > 0) read(0);
 
     // the middle's m largest: keys above `limit`, and the first `quota` that equal it
     const bool all = len <= e.budget;
@@ -68,9 +83,18 @@ paged_evict_select_kernel(EvictShape e) {
             shift -= bits;
             for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
             __syncthreads();
-            for (int i = first + tid; i < last; i += kSelThreads) {
-                const uint32_t k = order_key(sums[i]);
+            auto count = [&](float v) __attribute__((always_inline)) {
+                const uint32_t k = order_key(v);
                 if (pass == 0 || (k >> (shift + bits)) == above) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+            };
+            if constexpr (PER > 0) {
+#pragma unroll
+                for (int j = 0; j < HELD; ++j) {
+                    const int i = tid * per + j;
+                    if (j < per && i >= first && i < last) count(x[j]);
+                }
+            } else {
+                for (int i = first + tid; i < last; i += kSelThreads) count(sums[i]);
             }
             __syncthreads();
             // from the largest digit down: the digit in which the count reaches the quota
@@ -93,15 +117,14 @@ paged_evict_select_kernel(EvictShape e) {
 
     // places, in order: `sure` keys and equal keys counted together, 16 bits each
     uint32_t base_sure = 0, base_tie = 0;
-    for (int i0 = 0; i0 < len; i0 += kSelThreads * kPer) {
-        float x[kPer];
+    for (int i0 = 0; i0 < len; i0 += kSelThreads * per) {
+        if constexpr (PER == 0) read(i0);
         uint32_t sure = 0, tie = 0, mine = 0;
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int i = i0 + tid * kPer + j;
-            x[j] = i < len ? sums[i] : 0.f;
-            bool s = i < len, t = false;
-            if (!all && i >= first && i < last) {
+        for (int j = 0; j < HELD; ++j) {
+            const int i = i0 + tid * per + j;
+            bool s = j < per && i < len, t = false;
+            if (s && !all && i >= first && i < last) {
                 const uint32_t k = order_key(x[j]);
                 s = !none && k > limit;
                 t = !none && k == limit;
@@ -114,11 +137,11 @@ paged_evict_select_kernel(EvictShape e) {
         const uint32_t before = block_scan(mine, waves, total) - mine;
         uint32_t ns = base_sure + (before & 0xFFFFu), nt = base_tie + (before >> 16);
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
+        for (int j = 0; j < HELD; ++j) {
             const bool s = (sure >> j) & 1, t = (tie >> j) & 1;
             if (s || (t && nt < quota)) {
                 const uint32_t at = ns + min(nt, quota);
-                kept[at] = i0 + tid * kPer + j;
+                kept[at] = i0 + tid * per + j;
                 new_sums[at] = x[j];
             }
             ns += s;
@@ -162,7 +185,10 @@ paged_evict_move_kernel(PagedCache c, EvictShape e, FastDiv cpr, FastDiv budget,
 int paged_evict(const PagedCache& c, const EvictShape& e, hipStream_t s) {
     const int64_t rows = (int64_t)e.B * e.Hkv * e.budget, total = rows * (c.row_bytes / 16);
     if (total > 0x7fffff00) return fail(MYFA_E_UNSUPPORTED, "paged eviction: %lld chunks of 16 bytes in one call", (long long)total);
-    launch_kernel(paged_evict_select_kernel, dim3((unsigned)(e.B * e.Hkv)), dim3(kSelThreads), 0, s, e);
+    auto select = [&](auto kern) { launch_kernel(kern, dim3((unsigned)(e.B * e.Hkv)), dim3(kSelThreads), 0, s, e); };
+    if (e.cap <= 8 * kSelThreads) select(paged_evict_select_kernel<8>);
+    else if (e.cap <= 24 * kSelThreads) select(paged_evict_select_kernel<24>);
+    else select(paged_evict_select_kernel<0>);
     if (total > 0)
         launch_kernel(paged_evict_move_kernel, dim3((unsigned)cdiv(total, 256)), dim3(256), 0, s, c, e,
                       FastDiv((uint32_t)(c.row_bytes / 16)), FastDiv((uint32_t)e.budget), FastDiv((uint32_t)e.Hkv), (uint32_t)total);

@@ -333,12 +333,12 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
 
 // Few rows (see window_attn_common.h): 32 rows a workgroup, wave x takes tiles x, x + 4, ... of 32 keys.
 template <typename T, int D>
-__global__ void __launch_bounds__(256, 1)
+__global__ void __launch_bounds__(256, D * sizeof(T) <= 256 ? 2 : 1)
 window_bwd_dq_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
                          const T* __restrict__ dOg, const T* __restrict__ Og, const float* __restrict__ LSEg, float* __restrict__ st, T* __restrict__ dQg,
                          WindowShape w, int nqp, int64_t rows, int nqblk) {
     using R = TileReader<T, D>;
-    constexpr int BN = 32, NBUF = few_bufs<T, D>(), TILE_B = BN * R::RB, WAVE_B = few_wave_bytes<T, D>();
+    constexpr int BN = 32, TILE_B = BN * R::RB, WAVE_B = 2 * TILE_B;
     static_assert(WAVE_B >= 32 * D * 4, "a wave's sums fit its tiles");
     __shared__ __attribute__((aligned(1024))) char lds[4 * WAVE_B];
 
@@ -366,8 +366,7 @@ window_bwd_dq_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
         kfetch.fetch(Kh + (int64_t)k0 * w.ks[2], to, all, keep);
         vfetch.fetch(Vh + (int64_t)k0 * w.vs[2], to + TILE_B, all, keep);
     };
-#pragma unroll
-    for (int i = 0; i < NBUF; ++i) fetch(wave + 4 * i, own + i * 2 * TILE_B);
+    fetch(wave, own);
 
     typename R::frag qf[R::KS], of[R::KS];
     const int row = min(qrow, w.Nq - 1);
@@ -396,10 +395,9 @@ window_bwd_dq_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
 #pragma unroll
         for (int i = 0; i < 16; ++i) dq[db][i] = 0.f;
 
-    int buf = 0;
     for (int t = wave; t < ntiles; t += 4) {
         const int k0 = kt.first_key(t);
-        const char* Kb = own + buf * 2 * TILE_B;
+        const char* Kb = own;
         wave_fetched();
         f32x16 s, dp;
 #pragma unroll
@@ -414,8 +412,7 @@ window_bwd_dq_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
             sees.hide(s, kt, t, k0, k0 + 4 * h, w.sinks, 0.f);
         rd.add_transposed(Kb, 0, s, dq);
         wave_read();
-        fetch(t + 4 * NBUF, own + buf * 2 * TILE_B);
-        buf = NBUF == 2 ? buf ^ 1 : 0;
+        fetch(t + 4, own);
     }
 
     put_sums(reinterpret_cast<float*>(own), dq, r, h);
@@ -851,7 +848,7 @@ window_bwd_dkv_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, co
                           const T* __restrict__ dOg, const float* __restrict__ st, T* __restrict__ dKg, T* __restrict__ dVg,
                           float* __restrict__ parts, WindowShape w, int nqp, int64_t rows, int nsb, int ns) {
     using R = TileReader<T, D>;
-    constexpr int BQ = 32, NBUF = few_bufs<T, D>(), TILE_B = BQ * R::RB, WAVE_B = few_wave_bytes<T, D>();
+    constexpr int BQ = 32, NBUF = R::RB <= 256 ? 2 : 1, TILE_B = BQ * R::RB, WAVE_B = NBUF * 2 * TILE_B;
     constexpr int ODB = R::DB < 4 ? R::DB : 4, NC = R::DB / ODB, C = 32 * ODB;
     static_assert(WAVE_B >= 2 * 32 * C * 4, "a wave's sums fit its tiles");
     __shared__ __attribute__((aligned(1024))) char lds[4 * WAVE_B];
@@ -1024,7 +1021,7 @@ struct BwdPlan { bool few_q, few_k; int bk, nqp, nkblk, nsb, ns; int64_t rows, s
 // queries, at most 32 (the parts are written and read once more).
 BwdPlan bwd_plan(const WindowShape& w, int elem_size) {
     BwdPlan p;
-    p.few_q = few_queries(w, elem_size);
+    p.few_q = few_queries(w);
     p.few_k = few_keys(w, elem_size);
     p.bk = p.few_k ? 32 : 128;
     p.nqp = (int)cdiv(w.Nq, kStatPad) * kStatPad;

@@ -173,10 +173,10 @@ __device__ __forceinline__ void wave_read() { asm volatile("s_waitcnt lgkmcnt(0)
 
 // Few rows: a workgroup's four waves share 32 rows and deal the tiles among themselves, so that a launch has four
 // times the workgroups and each a quarter of the serial work; their float32 sums meet in LDS at the end.  A wave's
-// part of LDS holds kFewBufs pairs of 32-row tiles, and then its sums [32][C], 16-byte chunks swizzled so that
-// eight rows' chunks of one column lie on different banks.
-template <typename T, int D> constexpr int few_bufs() { return D * (int)sizeof(T) <= 256 ? 2 : 1; }
-template <typename T, int D> constexpr int few_wave_bytes() { return few_bufs<T, D>() * 2 * 32 * D * (int)sizeof(T); }
+// part of LDS holds a pair of 32-row tiles (dK, dV: two pairs where rows are up to 256 bytes), and then its sums
+// [32][C], 16-byte chunks swizzled so that eight rows' chunks of one column lie on different banks.  One pair
+// leaves room for a second workgroup on the CU, which hides more than a prefetch does (forward bf16 d 128, 128 blocks
+// of 128 rows: 11.9 us against 18.0 with two pairs).
 template <int C> __device__ __forceinline__ int sum_at(int row, int col) { return row * C + ((col >> 2) ^ (row & 7)) * 4; }
 template <int NDB> __device__ __forceinline__ void put_sums(float* to, const f32x16 (&acc)[NDB], int r, int h) {
 #pragma unroll
@@ -255,19 +255,17 @@ struct RowSees {
     }
 };
 
-// Whether a launch takes the few-rows kernels: while blocks of 128 rows leave CUs empty, and less of them where
-// a workgroup of the few-rows kernels fills a CU's LDS (16-bit rows of 256 bytes).  Measured, many / few, in us:
+// Whether a launch takes the few-rows kernels: while blocks of 128 rows leave CUs empty; dK, dV fewer of them where
+// one of its workgroups fills a CU's LDS (16-bit rows of 256 bytes).  Measured, many / few, in us:
 //   forward, bf16 d 64    128 blocks 15.7 / 7.9   192 15.5 / 11.6   256 15.7 / 13.4   512 18.2 / 22.1
-//            bf16 d 128    64 blocks 18.9 / 9.1   128 19.4 / 17.8   192 19.8 / 25.8
+//            bf16 d 128    64 blocks 18.9 / 8.7   128 19.6 / 11.9   192 19.7 / 17.7   256 19.9 / 20.6
 //            float32 d 64 128 blocks 43.1 / 25.3  192 43.1 / 36.6   256 43.8 / 48.0          dQ: alike
 //   dK, dV: what few saves of a whole backward, against blocks of 128 keys
 //            bf16 d 64     64 blocks 21 of 61     256 -35 to +61    512 3 of 65      1008 -3 of 138
 //            bf16 d 128    64 blocks 20 of 84     128 -3 of 76, -28 of 286           512 -27 of 105
 //            float32 d 64  64 blocks 168 of 310   256 200 of 1815   512 26 of 298    1008 -6 of 731
 // (float32 keeps gaining because the large kernel walks a whole group of heads in one workgroup.)
-inline bool few_queries(const WindowShape& w, int elem_size) {
-    return (int64_t)w.B * w.H * cdiv(w.Nq, 128) <= (elem_size == 2 && w.d > 64 ? 128 : 192);
-}
+inline bool few_queries(const WindowShape& w) { return (int64_t)w.B * w.H * cdiv(w.Nq, 128) <= 192; }
 inline bool few_keys(const WindowShape& w, int elem_size) {
     return (int64_t)w.B * w.Hkv * cdiv(w.Nk, 128) <= (elem_size == 4 ? 512 : w.d > 64 ? 64 : 192);
 }

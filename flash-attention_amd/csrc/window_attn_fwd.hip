@@ -342,11 +342,11 @@ window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
 
 // Few rows (see window_attn_common.h): 32 rows a workgroup, wave x takes tiles x, x + 4, ... of 32 keys.
 template <typename T, int D>
-__global__ void __launch_bounds__(256, D * sizeof(T) <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(256, D * sizeof(T) <= 256 ? 2 : 1)
 window_attn_fwd_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
                            T* __restrict__ Og, float* __restrict__ LSEg, WindowShape w, int nqblk) {
     using R = TileReader<T, D>;
-    constexpr int BN = 32, NBUF = few_bufs<T, D>(), TILE_B = BN * R::RB, WAVE_B = few_wave_bytes<T, D>();
+    constexpr int BN = 32, TILE_B = BN * R::RB, WAVE_B = 2 * TILE_B;
     static_assert(WAVE_B >= 32 * D * 4, "a wave's sums fit its tiles");
     __shared__ __attribute__((aligned(1024))) char lds[4 * WAVE_B];
     __shared__ float ml[4][2][32];
@@ -375,8 +375,7 @@ window_attn_fwd_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, c
         kfetch.fetch(Kh + (int64_t)k0 * w.ks[2], to, all, keep);
         vfetch.fetch(Vh + (int64_t)k0 * w.vs[2], to + TILE_B, all, keep);
     };
-#pragma unroll
-    for (int i = 0; i < NBUF; ++i) fetch(wave + 4 * i, own + i * 2 * TILE_B);
+    fetch(wave, own);
 
     typename R::frag qf[R::KS];
     {
@@ -397,10 +396,9 @@ window_attn_fwd_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, c
     float m = -INFINITY, l = 0.f;
     const float sl2 = w.scale * kLog2eW;
 
-    int buf = 0;
     for (int t = wave; t < ntiles; t += 4) {
         const int k0 = kt.first_key(t);
-        const char* Kb = own + buf * 2 * TILE_B;
+        const char* Kb = own;
         wave_fetched();
         f32x16 s;
 #pragma unroll
@@ -429,8 +427,7 @@ window_attn_fwd_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, c
             for (int i = 0; i < 16; ++i) o[db][i] *= alpha;
         rd.add_transposed(Kb + TILE_B, 0, s, o);
         wave_read();
-        fetch(t + 4 * NBUF, own + buf * 2 * TILE_B);
-        buf = NBUF == 2 ? buf ^ 1 : 0;
+        fetch(t + 4, own);
     }
 
     l = half_exchange_sum(l);
@@ -467,7 +464,7 @@ window_attn_fwd_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, c
 
 template <typename T>
 int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const WindowShape& w, hipStream_t s) {
-    const bool few = few_queries(w, (int)sizeof(T));
+    const bool few = few_queries(w);
     const int nqblk = (int)cdiv(w.Nq, few ? 32 : 128);
     const int64_t nwg = (int64_t)w.B * w.H * nqblk;
     if (nwg > 0x7fffffff) return fail(MYFA_E_UNSUPPORTED, "window attention: %lld query blocks", (long long)nwg);

@@ -239,6 +239,8 @@ EVICT = [
     ([100], 1, 16, 64, 40, 4, 8),
     ([100, 30, 0, 41, 40], 2, 16, 64, 40, 4, 8),
     ([9000, 300], 2, 24, 16, 777, 1, 100),
+    ([8192, 8191], 1, 16, 8, 3000, 0, 7),
+    ([30000], 1, 32, 8, 1111, 4, 64),
     ([5000], 1, 32, 8, 4999, 0, 0),
     ([64, 200], 3, 16, 80, 16, 4, 12),                 # nothing is left for the weights
     ([300], 2, 7, 64, 1, 0, 0),
