@@ -79,7 +79,8 @@ paged_decode_kernel(const T* __restrict__ Qg, PagedCache c, T* __restrict__ Og, 
     const int head0 = kvh * group + 16 * qt;
 
     const Seen sn = seen_of(w.lens[b], c.width * (int)c.page.d, w.window, w.sinks);
-    const int t0 = (int)((int64_t)sn.ntiles * part / ns), t1 = (int)((int64_t)sn.ntiles * (part + 1) / ns);
+    const int per = sn.ntiles / ns, more = sn.ntiles - per * ns;       // the first `more` shares have a tile more
+    const int t0 = per * part + min(part, more), t1 = t0 + per + (part < more ? 1 : 0);
 
     frag qf[KS];
     {

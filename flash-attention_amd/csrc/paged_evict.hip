@@ -186,8 +186,9 @@ int paged_evict(const PagedCache& c, const EvictShape& e, hipStream_t s) {
     const int64_t rows = (int64_t)e.B * e.Hkv * e.budget, total = rows * (c.row_bytes / 16);
     if (total > 0x7fffff00) return fail(MYFA_E_UNSUPPORTED, "paged eviction: %lld chunks of 16 bytes in one call", (long long)total);
     auto select = [&](auto kern) { launch_kernel(kern, dim3((unsigned)(e.B * e.Hkv)), dim3(kSelThreads), 0, s, e); };
-    if (e.cap <= 8 * kSelThreads) select(paged_evict_select_kernel<8>);
-    else if (e.cap <= 24 * kSelThreads) select(paged_evict_select_kernel<24>);
+    if (e.cap <= 2 * kSelThreads) select(paged_evict_select_kernel<2>);
+    else if (e.cap <= 8 * kSelThreads) select(paged_evict_select_kernel<8>);
+    else if (e.cap <= 16 * kSelThreads) select(paged_evict_select_kernel<16>);
     else select(paged_evict_select_kernel<0>);
     if (total > 0)
         launch_kernel(paged_evict_move_kernel, dim3((unsigned)cdiv(total, 256)), dim3(256), 0, s, c, e,

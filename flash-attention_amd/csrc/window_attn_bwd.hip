@@ -246,23 +246,22 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
     tile_ready();
 
     int cur = 0, nxt = 1, fre = 2;                 // K slots of tiles t, t + 1, t + 2
-    for (int t = 0; t < ntiles; ++t) {
-        const int k0 = kt.first_key(t);
+    // One tile: MASKED, or seen whole by all rows; `some`: the wave's rows see something of it; behind(): requests tile t + 2.
+    auto tile = [&](int t, int k0, bool some, auto masked_, auto&& behind) __attribute__((always_inline)) {
+        constexpr bool MASKED = decltype(masked_)::value != 0;
         const char* Kb = lds + cur * TILE_B;
         const char* Vb = lds + (3 + (t & 1)) * TILE_B;
-        const bool some = !(k0 > wave_hi || (k0 + BN <= wave_lo - w.window + 1 && k0 >= w.sinks));
-        const bool edge = !(k0 + BN - 1 <= wave_lo && wave_lo + 31 < kt.pz && (k0 >= wave_lo + 31 - w.window + 1 || k0 + BN <= w.sinks));
         f32x16 s[2], dp[2];
         typename M::vec8 sb[4];
         auto pds = [&](int kb, int i) __attribute__((always_inline)) {
             s[kb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], sl2, -lse2)) * dp[kb][i];
         };
         auto finish = [&](int kb) __attribute__((always_inline)) {
-            if (edge) sees.hide(s[kb], kt, t, k0, k0 + 32 * kb + 4 * h, w.sinks, 0.f);
+            if constexpr (MASKED) sees.hide(s[kb], kt, t, k0, k0 + 32 * kb + 4 * h, w.sinks, 0.f);
 #pragma unroll
             for (int i = 0; i < 16; ++i) sb[2 * kb + (i >> 3)][i & 7] = (T)s[kb][i];
         };
-        if (some) {
+        if (!MASKED || some) {
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -288,7 +287,7 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
             finish(0);
         }
         tile_ready();
-        if (some) {
+        if (!MASKED || some) {
             auto add = [&](auto kb_, auto&& after) __attribute__((always_inline)) {
                 constexpr int kb = decltype(kb_)::value;
                 mma_stream<2 * DB, FW>([&](auto ic) __attribute__((always_inline)) {
@@ -307,14 +306,41 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
             });
             finish(1);
             add(IC<1>{}, [&](auto ic) __attribute__((always_inline)) {
-                if constexpr (decltype(ic)::value == (2 * DB > FW ? 2 * DB - FW : 0)) fetch(t + 2, fre);
+                if constexpr (decltype(ic)::value == (2 * DB > FW ? 2 * DB - FW : 0)) behind();
             });
         } else {
-            fetch(t + 2, fre);
+            behind();
         }
         const int was = cur;
         cur = nxt; nxt = fre; fre = was;
+    };
+    auto masked_tiles = [&](int t0, int t1) __attribute__((always_inline)) {
+        for (int t = t0; t < t1; ++t) {
+            const int k0 = kt.first_key(t);
+            tile(t, k0, !(k0 > wave_hi || (k0 + BN <= wave_lo - w.window + 1 && k0 >= w.sinks)), IC<1>{},
+                 [&]() __attribute__((always_inline)) { fetch(t + 2, fre); });
+        }
+    };
+    const int f0 = kt.whole_from(w.window, 128), f1 = kt.whole_to(128);      // tiles that all rows see whole
+    masked_tiles(0, min(f0, ntiles));
+    if (f0 < f1) {
+        const T* kp = Kh + (int64_t)kt.first_key(f0 + 2) * w.ks[2];
+        const T* vp = Vh + (int64_t)kt.first_key(f0 + 2) * w.vs[2];
+        const int64_t kstep = BN * w.ks[2], vstep = BN * w.vs[2];
+        for (int t = f0; t < f1; ++t) {
+            tile(t, 0, true, IC<0>{}, [&]() __attribute__((always_inline)) {
+                if (t + 2 < f1) {
+                    kfetch.fetch(kp, lds + fre * TILE_B, true, [](int) { return true; });
+                    vfetch.fetch(vp, lds + (3 + (t & 1)) * TILE_B, true, [](int) { return true; });
+                } else {
+                    fetch(t + 2, fre);
+                }
+            });
+            kp += kstep;
+            vp += vstep;
+        }
     }
+    masked_tiles(min(max(f0, f1), ntiles), ntiles);
 
     if (qrow < w.Nq) {
         T* row = dQg + ((int64_t)bh * w.Nq + qrow) * w.d;
