@@ -18,9 +18,10 @@
 // Beyond 128 columns a workgroup of dK, dV keeps 128 columns of both (the accumulators and the fragments of
 // its keys fill the registers) and forms S and dP for each half again.
 // P and dS are rounded to the element type as operands; everything else is float32.  Rows and keys that
-// have no visible partner in the workgroup are fetched as zeros, so whatever stands there stays out.
+// have no visible partner in the workgroup are fetched as zeros, so whatever stands there stays out; what some of its
+// rows see and others do not: window_attn_exact.h.
 #include "attn_bwd_plan.h"
-#include "window_attn_common.h"
+#include "window_attn_exact.h"
 
 namespace myfa {
 namespace {
@@ -149,6 +150,14 @@ window_bwd_dq_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T
         }
     }
 
+    // (window_attn_exact.h)
+    const uint32_t redo = not_finite_rows(dq, live && finite(lse2) && finite(ndelta));
+    for (uint32_t left = redo; left != 0; left &= left - 1) {
+        const int x = __builtin_ctz(left), i = q0 + 32 * wave + x;
+        const int64_t at = ((int64_t)bh * w.Nq + i) * w.d;
+        exact_dq_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + i * w.qs[2], dOg + at, Kh, Vh, read_lane(lse2, x), read_lane(ndelta, x), dQg + at,
+                           w, i + kt.shift, lane);
+    }
     if (qrow < w.Nq) {
         T* row = dQg + ((int64_t)bh * w.Nq + qrow) * w.d;
         typedef T vec4 __attribute__((ext_vector_type(4)));
@@ -160,7 +169,7 @@ window_bwd_dq_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T
                 vec4 x;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = live ? (T)(dq[db][4 * g + j] * w.scale) : (T)0.f;
-                if (c < w.d) *reinterpret_cast<vec4*>(row + c) = x;
+                if (c < w.d && !(redo >> r & 1)) *reinterpret_cast<vec4*>(row + c) = x;
             }
     }
 }
@@ -342,6 +351,14 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
     }
     masked_tiles(min(max(f0, f1), ntiles), ntiles);
 
+    // (window_attn_exact.h)
+    const uint32_t redo = not_finite_rows(dq, live && finite(lse2) && finite(ndelta));
+    for (uint32_t left = redo; left != 0; left &= left - 1) {
+        const int x = __builtin_ctz(left), i = q0 + 32 * wave + x;
+        const int64_t at = ((int64_t)bh * w.Nq + i) * w.d;
+        exact_dq_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + i * w.qs[2], dOg + at, Kh, Vh, read_lane(lse2, x), read_lane(ndelta, x), dQg + at,
+                           w, i + kt.shift, lane);
+    }
     if (qrow < w.Nq) {
         T* row = dQg + ((int64_t)bh * w.Nq + qrow) * w.d;
 #pragma unroll
@@ -352,7 +369,7 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
                 typename M::vec4 x;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = live ? (T)(dq[db][4 * g + j] * w.scale) : (T)0.f;
-                if (c < w.d) *reinterpret_cast<typename M::vec4*>(row + c) = x;
+                if (c < w.d && !(redo >> r & 1)) *reinterpret_cast<typename M::vec4*>(row + c) = x;
             }
     }
 }
@@ -367,6 +384,7 @@ window_bwd_dq_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
     constexpr int BN = 32, TILE_B = BN * R::RB, WAVE_B = 2 * TILE_B;
     static_assert(WAVE_B >= 32 * D * 4, "a wave's sums fit its tiles");
     __shared__ __attribute__((aligned(1024))) char lds[4 * WAVE_B];
+    __shared__ uint32_t redo_of[4];
 
     const Ranked at_ = ranked(blockIdx.x, w.B * w.H);
     const int bh = at_.head, q0 = (nqblk - 1 - at_.rank) * 32;
@@ -442,7 +460,20 @@ window_bwd_dq_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
     }
 
     put_sums(reinterpret_cast<float*>(own), dq, r, h);
+    {
+        const uint32_t bad = not_finite_rows(dq, live && finite(stat.lse2) && finite(stat.ndelta));
+        if (lane == 0) redo_of[wave] = bad;
+    }
     __syncthreads();
+    const uint32_t redo = __builtin_amdgcn_readfirstlane(redo_of[0] | redo_of[1] | redo_of[2] | redo_of[3]);      // (window_attn_exact.h)
+    int turn = 0;
+    for (uint32_t left = redo; left != 0; left &= left - 1, ++turn) {
+        if ((turn & 3) != wave) continue;
+        const int x = __builtin_ctz(left);
+        const int64_t at = ((int64_t)bh * w.Nq + q0 + x) * w.d;
+        exact_dq_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + (q0 + x) * w.qs[2], dOg + at, Kh, Vh, read_lane(stat.lse2, x),
+                           read_lane(stat.ndelta, x), dQg + at, w, q0 + x + kt.shift, lane);
+    }
     typedef T vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int e = tid; e < 32 * D / 4; e += 256) {
@@ -455,11 +486,46 @@ window_bwd_dq_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
         vec4 y;
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = sees_any ? (T)(sum[j] * w.scale) : (T)0.f;
-        if (col < w.d) *reinterpret_cast<vec4*>(dQg + ((int64_t)bh * w.Nq + q0 + rw) * w.d + col) = y;
+        if (col < w.d && !(redo >> rw & 1)) *reinterpret_cast<vec4*>(dQg + ((int64_t)bh * w.Nq + q0 + rw) * w.d + col) = y;
     }
 }
 
 // ---------------------------------------------------------------- dK, dV
+// Where a workgroup of keys writes: the gradients, or, where its block is split, its part of them.
+template <typename T> struct KeyOut {
+    T *dk, *dv;                       // of the block's first key
+    float *pk, *pv;                   // null: not split
+};
+
+// The keys of `left` (window_attn_exact.h), bit x: key first + x, row x + base of the block; of every `turns` of them those with
+// turn `mine`; columns [c0, c1).  [j0, j1): the workgroup's tiles of BQ queries, nt a head from tile tq0 on.
+template <typename T, int D>
+__device__ __forceinline__ void exact_keys(uint32_t left, int turns, int mine, int first, int base, const WindowShape& w, int b, int kvh, int len,
+                                           int j0, int j1, int nt, int tq0, int BQ, const T* Qg, const T* Kg, const T* Vg, const T* dOg,
+                                           const float* st, int nqp, int64_t rows, const KeyOut<T>& to, int c0, int c1, int lane) {
+    const int shift = w.Nk - w.Nq, group = w.H / w.Hkv;
+    for (int turn = 0; left != 0; left &= left - 1, ++turn) {
+        if (turn % turns != mine) continue;
+        const int x = __builtin_ctz(left), key = first + x;
+        const int p_hi = key < w.sinks ? len - 1 : min(len - 1, key + w.window - 1);
+        ExactKey<T, D> e(Kg + b * w.ks[0] + kvh * w.ks[1] + key * w.ks[2], Vg + b * w.vs[0] + kvh * w.vs[1] + key * w.vs[2], w, lane);
+        for (int j = j0; j < j1; ++j) {
+            const int g = j / nt, i0 = (tq0 + j - g * nt) * BQ, head = kvh * group + g;
+            const int64_t bh = (int64_t)b * w.H + head;
+            const int from = max(i0, key - shift), to_i = min(i0 + BQ - 1, p_hi - shift);
+            for (int i = max(from, 0); i <= to_i; ++i)
+                e.add(Qg + b * w.qs[0] + head * w.qs[1] + i * w.qs[2], dOg + (bh * w.Nq + i) * w.d, st[bh * nqp + i], st[rows + bh * nqp + i]);
+        }
+        const int64_t at = (int64_t)(base + x) * w.d;
+        if (to.pk) {
+            e.dk.store(to.pk + at, w.scale, c0, c1, lane);
+            e.dv.store(to.pv + at, 1.f, c0, c1, lane);
+        } else {
+            e.dk.store(to.dk + at, w.scale, c0, c1, lane);
+            e.dv.store(to.dv + at, 1.f, c0, c1, lane);
+        }
+    }
+}
 template <typename T, int D>
 __global__ void __launch_bounds__(256, D * sizeof(T) <= 128 ? 2 : 1)
 window_bwd_dkv_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
@@ -513,6 +579,10 @@ window_bwd_dkv_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const 
             }
         }
     }
+    // Whether sums that are not finite get a second look (window_attn_exact.h): not where the key is so itself, or the first
+    // query that sees it.
+    const bool own = krow < w.Nk && (!seen || (finite_chunks<T>(kf) && finite_chunks<T>(vf) &&
+                     finite(st[rows + ((int64_t)b * w.H + kvh * group) * nqp + max(p_lo, shift) - shift])));
     const float sl2 = w.scale * kLog2eW;
 
     const R rd(lane);
@@ -582,7 +652,12 @@ window_bwd_dkv_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const 
         }
     }
 
-    if (krow >= w.Nk) return;
+    const KeyOut<T> to{dKg + ((int64_t)bg * w.Nk + k0) * w.d, dVg + ((int64_t)bg * w.Nk + k0) * w.d,
+                       split && ns > 1 ? parts + ((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 * w.d : nullptr,
+                       split && ns > 1 ? parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 + 1) * 128 * w.d : nullptr};
+    const uint32_t redo = not_finite_rows(dk, own) | not_finite_rows(dv, own);
+    exact_keys<T, D>(redo, 1, 0, k0 + 32 * wave, 32 * wave, w, b, kvh, len, j0, j1, nt, tq0, BQ, Qg, Kg, Vg, dOg, st, nqp, rows, to, col0, min(w.d, col0 + 32 * ODB), lane);
+    if (krow >= w.Nk || (redo >> r & 1)) return;
     typedef T vec4 __attribute__((ext_vector_type(4)));
     const int64_t at = ((int64_t)bg * w.Nk + krow) * w.d;
     float* pk = parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 + (krow - k0)) * w.d;
@@ -673,6 +748,10 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
     vec8 kf[KS], vf[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) { kf[ks] = __builtin_bit_cast(vec8, kf_[ks]); vf[ks] = __builtin_bit_cast(vec8, vf_[ks]); }
+    // Whether sums that are not finite get a second look (window_attn_exact.h): not where the key is so itself, or the first
+    // query that sees it.
+    const bool own = krow < w.Nk && (!seen || (finite_chunks<T>(kf_) && finite_chunks<T>(vf_) &&
+                     finite(st[rows + ((int64_t)b * w.H + kvh * group) * nqp + max(p_lo, shift) - shift])));
     const float sl2 = w.scale * kLog2eW;
 
     const R rd(lane);
@@ -842,7 +921,12 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // nothing in flight into an LDS that is given up
     }
 
-    if (krow >= w.Nk) return;
+    const KeyOut<T> to{dKg + ((int64_t)bg * w.Nk + k0) * w.d, dVg + ((int64_t)bg * w.Nk + k0) * w.d,
+                       split && ns > 1 ? parts + ((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 * w.d : nullptr,
+                       split && ns > 1 ? parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 + 1) * 128 * w.d : nullptr};
+    const uint32_t redo = not_finite_rows(dk, own) | not_finite_rows(dv, own);
+    exact_keys<T, D>(redo, 1, 0, k0 + 32 * wave, 32 * wave, w, b, kvh, len, j0, j1, nt, tq0, BQ, Qg, Kg, Vg, dOg, st, nqp, rows, to, 0, w.d, lane);
+    if (krow >= w.Nk || (redo >> r & 1)) return;
     const int64_t out = ((int64_t)bg * w.Nk + krow) * w.d;
     float* pk = parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 + (krow - k0)) * w.d;
 #pragma unroll
@@ -879,6 +963,7 @@ window_bwd_dkv_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, co
     static_assert(WAVE_B >= 2 * 32 * C * 4, "a wave's sums fit its tiles");
     __shared__ __attribute__((aligned(1024))) char lds[4 * WAVE_B];
     __shared__ __attribute__((aligned(16))) float stats[4][NBUF][2][32];
+    __shared__ uint32_t redo_of[4];
 
     const int lid = blockIdx.x / NC, col0 = ((int)blockIdx.x - lid * NC) * C;
     const Ranked at_ = ranked(lid, w.B * w.Hkv);
@@ -944,6 +1029,10 @@ window_bwd_dkv_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, co
             }
         }
     }
+    // Whether sums that are not finite get a second look (window_attn_exact.h): not where the key is so itself, or the first
+    // query that sees it.
+    const bool fit = krow < w.Nk && (!seen || (finite_chunks<T>(kf) && finite_chunks<T>(vf) &&
+                     finite(st[rows + ((int64_t)b * w.H + kvh * group) * nqp + max(p_lo, shift) - shift])));
     const float sl2 = w.scale * kLog2eW;
     f32x16 dk[ODB], dv[ODB];
 #pragma unroll
@@ -988,12 +1077,21 @@ window_bwd_dkv_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, co
 
     put_sums(reinterpret_cast<float*>(own), dk, r, h);
     put_sums(reinterpret_cast<float*>(own) + 32 * C, dv, r, h);
+    {
+        const uint32_t bad = not_finite_rows(dk, fit) | not_finite_rows(dv, fit);
+        if (lane == 0) redo_of[wave] = bad;
+    }
     __syncthreads();
+    const uint32_t redo = __builtin_amdgcn_readfirstlane(redo_of[0] | redo_of[1] | redo_of[2] | redo_of[3]);
+    const KeyOut<T> to{dKg + ((int64_t)bg * w.Nk + k0) * w.d, dVg + ((int64_t)bg * w.Nk + k0) * w.d,
+                       split && ns > 1 ? parts + ((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 32 * w.d : nullptr,
+                       split && ns > 1 ? parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 + 1) * 32 * w.d : nullptr};
+    exact_keys<T, D>(redo, 4, wave, k0, 0, w, b, kvh, len, j0, j1, nt, tq0, BQ, Qg, Kg, Vg, dOg, st, nqp, rows, to, col0, min(w.d, col0 + C), lane);
     typedef T vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int e = tid; e < 2 * 32 * C / 4; e += 256) {
         const int which = e / (32 * C / 4), rw = (e / (C / 4)) & 31, col = (e & (C / 4 - 1)) * 4, c = col0 + col;
-        if (k0 + rw >= w.Nk || c >= w.d) continue;
+        if (k0 + rw >= w.Nk || c >= w.d || (redo >> rw & 1)) continue;
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int x = 0; x < 4; ++x) sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * WAVE_B) + which * 32 * C + sum_at<C>(rw, col));

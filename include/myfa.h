@@ -291,8 +291,8 @@ int myfa_matmul_f32(const float* a, const float* b, float* c, int64_t m, int64_t
  *   window      >= 1 (more than Nk means Nk);  sinks >= 0;  scale > 0
  * Element types: MYFA_F16 and MYFA_BF16 with d a multiple of 8 up to 256, MYFA_F32 with d a multiple of 4 up to
  * 128; otherwise MYFA_E_UNSUPPORTED.  Statistics and sums are float32; P is rounded to the element type.
- * Keys and values that no row of 128 neighbouring queries sees, and what stands behind a sequence's length,
- * are not read into the products, whatever their bits are.
+ * What a row does not see, what stands behind a sequence's length included, does not reach it, whatever its bits
+ * are.  (Infinities and NaN that some rows see and their neighbours do not cost time: such rows are computed again.)
  * No counterpart in the reference, whose attention is unmasked (csrc/api.cpp:168-192).
  */
 int myfa_window_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* seq_lens,
@@ -303,7 +303,8 @@ int myfa_window_attn_fwd(const void* q, const void* k, const void* v, void* o, f
 /*
  * Gradients of myfa_window_attn_fwd.  o, lse: the forward's results; dout, dq: dense [B, H, Nq, d]; dk, dv: dense
  * [B, Hkv, Nk, d], summed over the query heads that share them; gradients of rows and keys that nothing sees or
- * that see nothing are 0.  `workspace`: myfa_window_attn_bwd_ws_bytes(...) bytes, 16-byte aligned, whose contents
+ * that see nothing are 0.  A row of q, k, v or dout that is not finite makes the gradients of the rows and keys it is
+ * seen with so, and no others.  `workspace`: myfa_window_attn_bwd_ws_bytes(...) bytes, 16-byte aligned, whose contents
  * before and after mean nothing; it must stay untouched until the call's work on `stream` has finished, and
  * calls that may overlap need one each.  No atomics: the result depends on the inputs alone.
  */

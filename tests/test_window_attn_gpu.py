@@ -166,6 +166,38 @@ def test_keys_before_every_window_may_hold_anything(mfa):
         ref.check(name, got[name], want[name])
 
 
+@pytest.mark.parametrize("what", ["v", "k", "q", "dout"])
+@pytest.mark.parametrize("shape", [(1, 4, 2, 260, 260, 64, 20, 0, BF16), (1, 4, 2, 150, 260, 128, 20, 3, F16), (1, 2, 1, 200, 200, 64, 20, 2, F32),
+                                   (1, 2, 1, 180, 180, 192, 20, 2, BF16),                                       # few rows
+                                   (1, 128, 64, 260, 260, 64, 20, 3, BF16), (1, 100, 100, 260, 260, 128, 20, 0, BF16),  # many
+                                   (1, 100, 100, 260, 260, 64, 20, 3, F32), (1, 100, 100, 200, 200, 160, 20, 2, F16)],
+                         ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+def test_what_a_row_does_not_see_may_hold_anything(mfa, shape, what):
+    """A key, value, query or gradient row that is infinite or NaN reaches what sees it, and nothing else, though tiles hold
+    both."""
+    B, H, G, nq, nk, d, window, sinks, dtype = shape
+    q, k, v, dout = _inputs(B, H, G, nq, nk, d, dtype, 4)
+    vis = _visible(B, nq, nk, window, sinks, None)
+    want = ref.attention(q, k, v, vis, 0.125, dtype, dout)
+    at = 141                                             # a position
+    row_bad, key_bad = torch.zeros(nq, dtype=torch.bool), torch.zeros(nk, dtype=torch.bool)
+    if what in "kv":
+        {"k": k, "v": v}[what][:, :, at] = float("nan") if what == "k" else float("inf")
+        row_bad = vis[0][:, at].clone()
+    else:
+        {"q": q, "dout": dout}[what][:, :, at - (nk - nq)] = float("nan")
+        row_bad[at - (nk - nq)] = True
+    key_bad = vis[0][row_bad].any(0)
+    out_bad = row_bad if what != "dout" else torch.zeros_like(row_bad)
+    assert row_bad.any() and not row_bad.all() and not key_bad.all()
+    got = _run(mfa, *(t.cuda() for t in (q, k, v, dout)), window, sinks, 0.125, None)
+    for name, keep in (("out", ~out_bad), ("dq", ~row_bad), ("dk", ~key_bad), ("dv", ~key_bad)):
+        ref.check(name, got[name][:, :, keep.cuda()], tuple(t[:, :, keep] for t in want[name]))
+    if out_bad.any():
+        assert not torch.isfinite(got["out"][:, :, out_bad.cuda()]).any()
+    assert torch.isnan(got["dq"][:, :, row_bad.cuda()]).any(-1).all()
+
+
 def test_strided_views(mfa):
     """(B, N, H, d) layouts and slices of one fused projection give what dense copies give, bit for bit."""
     torch.manual_seed(0)
