@@ -3,9 +3,6 @@
 The reference's attention sees every key (csrc/api.cpp:168-192); this is the form that decoders with long
 contexts use, beside flash_attn_fwd / flash_attn_bwd / flash_attn_func and in their manner.
 """
-import torch
-from torch.autograd.function import once_differentiable
-
 from . import _host
 
 
@@ -31,22 +28,6 @@ def window_attn_bwd(dout, q, k, v, out, lse, window, sinks=0, scale=1.0, seq_len
     return _host.window_attn_bwd(dout, q, k, v, out, lse, window, sinks, scale, seq_lens)
 
 
-class _WindowAttnFunc(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, window, sinks, scale, seq_lens):
-        out, lse = window_attn_fwd(q, k, v, window, sinks=sinks, scale=scale, return_lse=True, seq_lens=seq_lens)
-        ctx.save_for_backward(q, k, v, out, lse, seq_lens)
-        ctx.window, ctx.sinks, ctx.scale = window, sinks, scale
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        q, k, v, out, lse, seq_lens = ctx.saved_tensors
-        dq, dk, dv = window_attn_bwd(dout.contiguous(), q, k, v, out, lse, ctx.window, sinks=ctx.sinks, scale=ctx.scale, seq_lens=seq_lens)
-        return dq, dk, dv, None, None, None, None
-
-
 def window_attn_func(q, k, v, window, sinks=0, scale=1.0, seq_lens=None):
-    """window_attn_fwd with autograd support, for everything it serves."""
-    return _WindowAttnFunc.apply(q, k, v, window, sinks, scale, seq_lens)
+    """window_attn_fwd with autograd support (once differentiable), for everything it serves."""
+    return _host.window_attn_func(q, k, v, window, sinks, scale, seq_lens)

@@ -252,6 +252,33 @@ def test_autograd(mfa):
         assert torch.equal(g, want[name]), name
 
 
+def test_autograd_at_its_edges(mfa):
+    q, k, v, dout = (t.cuda() for t in _inputs(1, 4, 2, 40, 64, 60, BF16, 7))               # (a head dim that is padded)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    out = mfa.window_attn_func(*leaves, 20, scale=0.125)
+    want = torch.autograd.grad(out, leaves, dout, retain_graph=True)
+    moved = torch.empty(dout.numel() + 1, dtype=dout.dtype, device="cuda")[1:].view(dout.shape)
+    moved.copy_(dout)                                                                       # dense, off the 16-byte grid
+    for a, b in zip(torch.autograd.grad(out, leaves, moved, retain_graph=True), want):
+        assert torch.equal(a, b)
+    ones = torch.autograd.grad(out, leaves, torch.ones_like(out), retain_graph=True)
+    for a, b in zip(torch.autograd.grad(out.sum(), leaves, retain_graph=True), ones):      # an expanded gradient
+        assert torch.equal(a, b)
+    for a, b in zip(torch.autograd.grad(out, leaves[1:2], dout, retain_graph=True), want[1:2]):
+        assert torch.equal(a, b)
+    twice = torch.autograd.grad(out, leaves, dout, retain_graph=True, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(twice, want))
+    with pytest.raises(RuntimeError, match="once"):
+        twice[0].sum().backward()
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(twice[0].sum(), leaves)
+    assert not mfa.window_attn_func(q, k, v, 20).requires_grad
+    with torch.no_grad():
+        leaves[0].add_(1)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(out, leaves, dout)
+
+
 def test_other_stream(mfa):
     q, k, v, dout = (t.cuda() for t in _inputs(1, 4, 2, 500, 500, 128, BF16, 8))
     want = _run(mfa, q, k, v, dout, 100, 4, 0.1, None)
