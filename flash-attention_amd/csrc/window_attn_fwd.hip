@@ -166,6 +166,11 @@ window_attn_fwd_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
 //   Weights up to 2^8 are rounded with the same relative error, and neither the search for the maximum nor the
 //   rescale of O, 64 multiplications a lane, is in most tiles.
 //   The tiles that every row of the workgroup sees whole run in a loop without masks, bounds or tile arithmetic.
+// Measured (bf16, d 128): 16 heads of 16384 positions, window 4096: 452 us, 1065 TFLOP/s of what is seen, where a
+// library product of 8192^3 reaches 1194; B 4, 32 heads of 4096 positions, window 1024: 295 us, 817 (a tenth of the work
+// is in tiles that the masks halve).  Bound by the matrix pipe at the clock that the power limit leaves it: on operands
+// that are all ones the first takes 358 us.  Forming each half of a tile's weights beside the products of the other
+// half changed neither (460 against 459 us, all ones 360 against 358): the two workgroups of a CU do that already.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 2)
 window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
