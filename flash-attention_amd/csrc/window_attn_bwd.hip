@@ -154,14 +154,7 @@ window_bwd_dq_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T
         }
     }
 
-    // (window_attn_exact.h)
     const uint32_t redo = not_finite_rows(dq, live && finite(lse2) && finite(ndelta));
-    for (uint32_t left = redo; left != 0; left &= left - 1) {
-        const int x = __builtin_ctz(left), i = q0 + 32 * wave + x;
-        const int64_t at = ((int64_t)bh * w.Nq + i) * w.d;
-        exact_dq_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + i * w.qs[2], dOg + at, Kh, Vh, read_lane(lse2, x), read_lane(ndelta, x), dQg + at,
-                           w, i + kt.shift, lane);
-    }
     if (qrow < w.Nq) {
         T* row = dQg + ((int64_t)bh * w.Nq + qrow) * w.d;
         typedef T vec4 __attribute__((ext_vector_type(4)));
@@ -173,8 +166,18 @@ window_bwd_dq_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T
                 vec4 x;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = live ? (T)(dq[db][4 * g + j] * w.scale) : (T)0.f;
-                if (c < w.d && !(redo >> r & 1)) *reinterpret_cast<vec4*>(row + c) = x;
+                if (c < w.d) *reinterpret_cast<vec4*>(row + c) = x;
             }
+    }
+    if (redo != 0) {                                        // (window_attn_exact.h)
+        const uint32_t cols = hidden_for_dq<T, D>(kt, w, q0 + 32 * wave + kt.shift, Kh, Vh, lane);
+        stored();
+        for (uint32_t left = any_lane(cols != 0) ? redo : 0; left != 0; left &= left - 1) {
+            const int x = __builtin_ctz(left), i = q0 + 32 * wave + x;
+            const int64_t at = ((int64_t)bh * w.Nq + i) * w.d;
+            exact_dq_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + i * w.qs[2], dOg + at, Kh, Vh, read_lane(lse2, x), read_lane(ndelta, x), dQg + at,
+                               w, i + kt.shift, cols, lane);
+        }
     }
 }
 
@@ -355,14 +358,7 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
     }
     masked_tiles(min(max(f0, f1), ntiles), ntiles);
 
-    // (window_attn_exact.h)
     const uint32_t redo = not_finite_rows(dq, live && finite(lse2) && finite(ndelta));
-    for (uint32_t left = redo; left != 0; left &= left - 1) {
-        const int x = __builtin_ctz(left), i = q0 + 32 * wave + x;
-        const int64_t at = ((int64_t)bh * w.Nq + i) * w.d;
-        exact_dq_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + i * w.qs[2], dOg + at, Kh, Vh, read_lane(lse2, x), read_lane(ndelta, x), dQg + at,
-                           w, i + kt.shift, lane);
-    }
     if (qrow < w.Nq) {
         T* row = dQg + ((int64_t)bh * w.Nq + qrow) * w.d;
 #pragma unroll
@@ -373,8 +369,18 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
                 typename M::vec4 x;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = live ? (T)(dq[db][4 * g + j] * w.scale) : (T)0.f;
-                if (c < w.d && !(redo >> r & 1)) *reinterpret_cast<typename M::vec4*>(row + c) = x;
+                if (c < w.d) *reinterpret_cast<typename M::vec4*>(row + c) = x;
             }
+    }
+    if (redo != 0) {                                        // (window_attn_exact.h)
+        const uint32_t cols = hidden_for_dq<T, D>(kt, w, q0 + 32 * wave + kt.shift, Kh, Vh, lane);
+        stored();
+        for (uint32_t left = any_lane(cols != 0) ? redo : 0; left != 0; left &= left - 1) {
+            const int x = __builtin_ctz(left), i = q0 + 32 * wave + x;
+            const int64_t at = ((int64_t)bh * w.Nq + i) * w.d;
+            exact_dq_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + i * w.qs[2], dOg + at, Kh, Vh, read_lane(lse2, x), read_lane(ndelta, x), dQg + at,
+                               w, i + kt.shift, cols, lane);
+        }
     }
 }
 
@@ -469,15 +475,7 @@ window_bwd_dq_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
         if (lane == 0) redo_of[wave] = bad;
     }
     __syncthreads();
-    const uint32_t redo = __builtin_amdgcn_readfirstlane(redo_of[0] | redo_of[1] | redo_of[2] | redo_of[3]);      // (window_attn_exact.h)
-    int turn = 0;
-    for (uint32_t left = redo; left != 0; left &= left - 1, ++turn) {
-        if ((turn & 3) != wave) continue;
-        const int x = __builtin_ctz(left);
-        const int64_t at = ((int64_t)bh * w.Nq + q0 + x) * w.d;
-        exact_dq_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + (q0 + x) * w.qs[2], dOg + at, Kh, Vh, read_lane(stat.lse2, x),
-                           read_lane(stat.ndelta, x), dQg + at, w, q0 + x + kt.shift, lane);
-    }
+    const uint32_t redo = __builtin_amdgcn_readfirstlane(redo_of[0] | redo_of[1] | redo_of[2] | redo_of[3]);
     typedef T vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int e = tid; e < 32 * D / 4; e += 256) {
@@ -490,7 +488,20 @@ window_bwd_dq_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
         vec4 y;
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = sees_any ? (T)(sum[j] * w.scale) : (T)0.f;
-        if (col < w.d && !(redo >> rw & 1)) *reinterpret_cast<vec4*>(dQg + ((int64_t)bh * w.Nq + q0 + rw) * w.d + col) = y;
+        if (col < w.d) *reinterpret_cast<vec4*>(dQg + ((int64_t)bh * w.Nq + q0 + rw) * w.d + col) = y;
+    }
+    if (redo != 0) {                                        // (window_attn_exact.h)
+        const uint32_t cols = hidden_for_dq<T, D>(kt, w, q0 + kt.shift, Kh, Vh, lane);
+        stored();
+        __syncthreads();
+        int turn = 0;
+        for (uint32_t left = any_lane(cols != 0) ? redo : 0; left != 0; left &= left - 1, ++turn) {
+            if ((turn & 3) != wave) continue;
+            const int x = __builtin_ctz(left);
+            const int64_t at = ((int64_t)bh * w.Nq + q0 + x) * w.d;
+            exact_dq_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + (q0 + x) * w.qs[2], dOg + at, Kh, Vh, read_lane(stat.lse2, x),
+                               read_lane(stat.ndelta, x), dQg + at, w, q0 + x + kt.shift, cols, lane);
+        }
     }
 }
 
@@ -501,32 +512,53 @@ template <typename T> struct KeyOut {
     float *pk, *pv;                   // null: not split
 };
 
-// The keys of `left` (window_attn_exact.h), bit x: key first + x, row x + base of the block; of every `turns` of them those with
-// turn `mine`; columns [c0, c1).  [j0, j1): the workgroup's tiles of BQ queries, nt a head from tile tq0 on.
+// The second look (window_attn_exact.h) of a wave at its keys first .. first + 31, rows base .. of the block: those of `left`, bit x: key
+// first + x, of every `turns` of them the ones with turn `mine`; columns [c0, c1).  The workgroup's tiles are [j0, j1), of BQ
+// queries, nt a head from tile tq0 on; their queries at positions outside [pa, pz) were fetched as zeros.
 template <typename T, int D>
 __device__ __forceinline__ void exact_keys(uint32_t left, int turns, int mine, int first, int base, const WindowShape& w, int b, int kvh, int len,
-                                           int j0, int j1, int nt, int tq0, int BQ, const T* Qg, const T* Kg, const T* Vg, const T* dOg,
-                                           const float* st, int nqp, int64_t rows, const KeyOut<T>& to, int c0, int c1, int lane) {
-    const int shift = w.Nk - w.Nq, group = w.H / w.Hkv;
+                                           int pa, int pz, int j0, int j1, int nt, int tq0, int BQ, const T* Qg, const T* Kg, const T* Vg,
+                                           const T* dOg, const float* st, int nqp, int64_t rows, const KeyOut<T>& to, int c0, int c1, int lane) {
+    using L = LaneRow<T, D>;
+    const int shift = w.Nk - w.Nq, group = w.H / w.Hkv, last = first + 31;
+    // columns that hidden queries reach: of dV where dO is not finite; of dK where Q is not, and all where dO or delta is not
+    uint32_t ck = 0, cv = 0;
+    for (int j = j0; j < j1; ++j) {
+        const int g = j / nt, i0 = (tq0 + j - g * nt) * BQ, head = kvh * group + g, pt = i0 + shift;
+        const int64_t bh = (int64_t)b * w.H + head;
+        if (pt >= last && pt + BQ <= len && last < w.Nk && (last < w.sinks || pt + BQ - 1 < first + w.window)) continue;
+        for (int i = i0; i < i0 + BQ; ++i) {
+            if (!finite(st[rows + bh * nqp + i])) ck = L::all(w.d, lane);
+            if (i + shift < pa || i + shift >= pz) continue;
+            const uint32_t bad = L(dOg + (bh * w.Nq + i) * w.d, w.d, lane).not_finite();
+            cv |= bad;
+            ck |= any_lane(bad != 0) ? L::all(w.d, lane) : L(Qg + b * w.qs[0] + head * w.qs[1] + i * w.qs[2], w.d, lane).not_finite();
+        }
+    }
+    if (!any_lane((ck | cv) != 0)) return;
     for (int turn = 0; left != 0; left &= left - 1, ++turn) {
         if (turn % turns != mine) continue;
         const int x = __builtin_ctz(left), key = first + x;
         const int p_hi = key < w.sinks ? len - 1 : min(len - 1, key + w.window - 1);
         ExactKey<T, D> e(Kg + b * w.ks[0] + kvh * w.ks[1] + key * w.ks[2], Vg + b * w.vs[0] + kvh * w.vs[1] + key * w.vs[2], w, lane);
-        for (int j = j0; j < j1; ++j) {
+        bool more = true;
+        for (int j = j0; j < j1 && more; ++j) {
             const int g = j / nt, i0 = (tq0 + j - g * nt) * BQ, head = kvh * group + g;
             const int64_t bh = (int64_t)b * w.H + head;
             const int from = max(i0, key - shift), to_i = min(i0 + BQ - 1, p_hi - shift);
-            for (int i = max(from, 0); i <= to_i; ++i)
-                e.add(Qg + b * w.qs[0] + head * w.qs[1] + i * w.qs[2], dOg + (bh * w.Nq + i) * w.d, st[bh * nqp + i], st[rows + bh * nqp + i]);
+            for (int i = max(from, 0); i <= to_i && more; i += kAtOnce) {
+                e.add(Qg + b * w.qs[0] + head * w.qs[1] + i * w.qs[2], w.qs[2], dOg + (bh * w.Nq + i) * w.d, st + bh * nqp + i,
+                      st + rows + bh * nqp + i, min(kAtOnce, to_i + 1 - i));
+                more = any_lane(((ck & ~e.dk.not_finite()) | (cv & ~e.dv.not_finite())) != 0);
+            }
         }
         const int64_t at = (int64_t)(base + x) * w.d;
         if (to.pk) {
-            e.dk.store(to.pk + at, w.scale, c0, c1, lane);
-            e.dv.store(to.pv + at, 1.f, c0, c1, lane);
+            e.dk.store(to.pk + at, w.scale, ck, c0, c1, lane);
+            e.dv.store(to.pv + at, 1.f, cv, c0, c1, lane);
         } else {
-            e.dk.store(to.dk + at, w.scale, c0, c1, lane);
-            e.dv.store(to.dv + at, 1.f, c0, c1, lane);
+            e.dk.store(to.dk + at, w.scale, ck, c0, c1, lane);
+            e.dv.store(to.dv + at, 1.f, cv, c0, c1, lane);
         }
     }
 }
@@ -583,10 +615,6 @@ window_bwd_dkv_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const 
             }
         }
     }
-    // Whether sums that are not finite get a second look (window_attn_exact.h): not where the key is so itself, or the first
-    // query that sees it.
-    const bool own = krow < w.Nk && (!seen || (finite_chunks<T>(kf) && finite_chunks<T>(vf) &&
-                     finite(st[rows + ((int64_t)b * w.H + kvh * group) * nqp + max(p_lo, shift) - shift])));
     const float sl2 = w.scale * kLog2eW;
 
     const R rd(lane);
@@ -656,35 +684,40 @@ window_bwd_dkv_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const 
         }
     }
 
-    const KeyOut<T> to{dKg + ((int64_t)bg * w.Nk + k0) * w.d, dVg + ((int64_t)bg * w.Nk + k0) * w.d,
-                       split && ns > 1 ? parts + ((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 * w.d : nullptr,
-                       split && ns > 1 ? parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 + 1) * 128 * w.d : nullptr};
-    const uint32_t redo = not_finite_rows(dk, own) | not_finite_rows(dv, own);
-    exact_keys<T, D>(redo, 1, 0, k0 + 32 * wave, 32 * wave, w, b, kvh, len, j0, j1, nt, tq0, BQ, Qg, Kg, Vg, dOg, st, nqp, rows, to, col0, min(w.d, col0 + 32 * ODB), lane);
-    if (krow >= w.Nk || (redo >> r & 1)) return;
-    typedef T vec4 __attribute__((ext_vector_type(4)));
-    const int64_t at = ((int64_t)bg * w.Nk + krow) * w.d;
-    float* pk = parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 + (krow - k0)) * w.d;
+    const uint32_t redo = not_finite_rows(dk, krow < w.Nk) | not_finite_rows(dv, krow < w.Nk);
+    if (krow < w.Nk) {
+        typedef T vec4 __attribute__((ext_vector_type(4)));
+        const int64_t at = ((int64_t)bg * w.Nk + krow) * w.d;
+        float* pk = parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 + (krow - k0)) * w.d;
 #pragma unroll
-    for (int db = 0; db < ODB; ++db)
+        for (int db = 0; db < ODB; ++db)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int c = col0 + 32 * db + 8 * g + 4 * h;
-            if (c >= w.d) continue;
-            f32x4 xk, xv;
+            for (int g = 0; g < 4; ++g) {
+                const int c = col0 + 32 * db + 8 * g + 4 * h;
+                if (c >= w.d) continue;
+                f32x4 xk, xv;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { xk[e] = dk[db][4 * g + e] * w.scale; xv[e] = dv[db][4 * g + e]; }
-            if (split && ns > 1) {
-                *reinterpret_cast<f32x4*>(pk + c) = xk;
-                *reinterpret_cast<f32x4*>(pk + (int64_t)128 * w.d + c) = xv;
-            } else {
-                vec4 yk, yv;
+                for (int e = 0; e < 4; ++e) { xk[e] = dk[db][4 * g + e] * w.scale; xv[e] = dv[db][4 * g + e]; }
+                if (split && ns > 1) {
+                    *reinterpret_cast<f32x4*>(pk + c) = xk;
+                    *reinterpret_cast<f32x4*>(pk + (int64_t)128 * w.d + c) = xv;
+                } else {
+                    vec4 yk, yv;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { yk[e] = (T)xk[e]; yv[e] = (T)xv[e]; }
-                *reinterpret_cast<vec4*>(dKg + at + c) = yk;
-                *reinterpret_cast<vec4*>(dVg + at + c) = yv;
+                    for (int e = 0; e < 4; ++e) { yk[e] = (T)xk[e]; yv[e] = (T)xv[e]; }
+                    *reinterpret_cast<vec4*>(dKg + at + c) = yk;
+                    *reinterpret_cast<vec4*>(dVg + at + c) = yv;
+                }
             }
-        }
+    }
+    if (redo != 0) {                                        // (window_attn_exact.h)
+        const KeyOut<T> to{dKg + ((int64_t)bg * w.Nk + k0) * w.d, dVg + ((int64_t)bg * w.Nk + k0) * w.d,
+                           split && ns > 1 ? parts + ((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 * w.d : nullptr,
+                           split && ns > 1 ? parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 + 1) * 128 * w.d : nullptr};
+        stored();
+        exact_keys<T, D>(redo, 1, 0, k0 + 32 * wave, 32 * wave, w, b, kvh, len, pa, pz, j0, j1, nt, tq0, BQ, Qg, Kg, Vg, dOg, st, nqp, rows, to,
+                         col0, min(w.d, col0 + 32 * ODB), lane);
+    }
 }
 
 // dK, dV for 16-bit elements and up to 128 columns: one wave per SIMD with the keys' fragments and both
@@ -752,10 +785,6 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
     vec8 kf[KS], vf[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) { kf[ks] = __builtin_bit_cast(vec8, kf_[ks]); vf[ks] = __builtin_bit_cast(vec8, vf_[ks]); }
-    // Whether sums that are not finite get a second look (window_attn_exact.h): not where the key is so itself, or the first
-    // query that sees it.
-    const bool own = krow < w.Nk && (!seen || (finite_chunks<T>(kf_) && finite_chunks<T>(vf_) &&
-                     finite(st[rows + ((int64_t)b * w.H + kvh * group) * nqp + max(p_lo, shift) - shift])));
     const float sl2 = w.scale * kLog2eW;
 
     const R rd(lane);
@@ -925,34 +954,39 @@ window_bwd_dkv16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, cons
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // nothing in flight into an LDS that is given up
     }
 
-    const KeyOut<T> to{dKg + ((int64_t)bg * w.Nk + k0) * w.d, dVg + ((int64_t)bg * w.Nk + k0) * w.d,
-                       split && ns > 1 ? parts + ((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 * w.d : nullptr,
-                       split && ns > 1 ? parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 + 1) * 128 * w.d : nullptr};
-    const uint32_t redo = not_finite_rows(dk, own) | not_finite_rows(dv, own);
-    exact_keys<T, D>(redo, 1, 0, k0 + 32 * wave, 32 * wave, w, b, kvh, len, j0, j1, nt, tq0, BQ, Qg, Kg, Vg, dOg, st, nqp, rows, to, 0, w.d, lane);
-    if (krow >= w.Nk || (redo >> r & 1)) return;
-    const int64_t out = ((int64_t)bg * w.Nk + krow) * w.d;
-    float* pk = parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 + (krow - k0)) * w.d;
+    const uint32_t redo = not_finite_rows(dk, krow < w.Nk) | not_finite_rows(dv, krow < w.Nk);
+    if (krow < w.Nk) {
+        const int64_t out = ((int64_t)bg * w.Nk + krow) * w.d;
+        float* pk = parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 + (krow - k0)) * w.d;
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int c = 32 * db + 8 * g + 4 * h;
-            if (c >= w.d) continue;
-            f32x4 xk, xv;
+            for (int g = 0; g < 4; ++g) {
+                const int c = 32 * db + 8 * g + 4 * h;
+                if (c >= w.d) continue;
+                f32x4 xk, xv;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) { xk[e] = dk[db][4 * g + e] * w.scale; xv[e] = dv[db][4 * g + e]; }
-            if (split && ns > 1) {
-                *reinterpret_cast<f32x4*>(pk + c) = xk;
-                *reinterpret_cast<f32x4*>(pk + (int64_t)128 * w.d + c) = xv;
-            } else {
-                vec4 yk, yv;
+                for (int e = 0; e < 4; ++e) { xk[e] = dk[db][4 * g + e] * w.scale; xv[e] = dv[db][4 * g + e]; }
+                if (split && ns > 1) {
+                    *reinterpret_cast<f32x4*>(pk + c) = xk;
+                    *reinterpret_cast<f32x4*>(pk + (int64_t)128 * w.d + c) = xv;
+                } else {
+                    vec4 yk, yv;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { yk[e] = (T)xk[e]; yv[e] = (T)xv[e]; }
-                *reinterpret_cast<vec4*>(dKg + out + c) = yk;
-                *reinterpret_cast<vec4*>(dVg + out + c) = yv;
+                    for (int e = 0; e < 4; ++e) { yk[e] = (T)xk[e]; yv[e] = (T)xv[e]; }
+                    *reinterpret_cast<vec4*>(dKg + out + c) = yk;
+                    *reinterpret_cast<vec4*>(dVg + out + c) = yv;
+                }
             }
-        }
+    }
+    if (redo != 0) {                                        // (window_attn_exact.h)
+        const KeyOut<T> to{dKg + ((int64_t)bg * w.Nk + k0) * w.d, dVg + ((int64_t)bg * w.Nk + k0) * w.d,
+                           split && ns > 1 ? parts + ((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 128 * w.d : nullptr,
+                           split && ns > 1 ? parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 + 1) * 128 * w.d : nullptr};
+        stored();
+        exact_keys<T, D>(redo, 1, 0, k0 + 32 * wave, 32 * wave, w, b, kvh, len, pa, pz, j0, j1, nt, tq0, BQ, Qg, Kg, Vg, dOg, st, nqp, rows, to,
+                         0, w.d, lane);
+    }
 }
 
 // Few rows (see window_attn_common.h): 32 keys a workgroup, wave x takes every fourth of the query tiles of 32.
@@ -1033,10 +1067,6 @@ window_bwd_dkv_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, co
             }
         }
     }
-    // Whether sums that are not finite get a second look (window_attn_exact.h): not where the key is so itself, or the first
-    // query that sees it.
-    const bool fit = krow < w.Nk && (!seen || (finite_chunks<T>(kf) && finite_chunks<T>(vf) &&
-                     finite(st[rows + ((int64_t)b * w.H + kvh * group) * nqp + max(p_lo, shift) - shift])));
     const float sl2 = w.scale * kLog2eW;
     f32x16 dk[ODB], dv[ODB];
 #pragma unroll
@@ -1082,20 +1112,16 @@ window_bwd_dkv_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, co
     put_sums(reinterpret_cast<float*>(own), dk, r, h);
     put_sums(reinterpret_cast<float*>(own) + 32 * C, dv, r, h);
     {
-        const uint32_t bad = not_finite_rows(dk, fit) | not_finite_rows(dv, fit);
+        const uint32_t bad = not_finite_rows(dk, krow < w.Nk) | not_finite_rows(dv, krow < w.Nk);
         if (lane == 0) redo_of[wave] = bad;
     }
     __syncthreads();
     const uint32_t redo = __builtin_amdgcn_readfirstlane(redo_of[0] | redo_of[1] | redo_of[2] | redo_of[3]);
-    const KeyOut<T> to{dKg + ((int64_t)bg * w.Nk + k0) * w.d, dVg + ((int64_t)bg * w.Nk + k0) * w.d,
-                       split && ns > 1 ? parts + ((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 32 * w.d : nullptr,
-                       split && ns > 1 ? parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 + 1) * 32 * w.d : nullptr};
-    exact_keys<T, D>(redo, 4, wave, k0, 0, w, b, kvh, len, j0, j1, nt, tq0, BQ, Qg, Kg, Vg, dOg, st, nqp, rows, to, col0, min(w.d, col0 + C), lane);
     typedef T vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int e = tid; e < 2 * 32 * C / 4; e += 256) {
         const int which = e / (32 * C / 4), rw = (e / (C / 4)) & 31, col = (e & (C / 4 - 1)) * 4, c = col0 + col;
-        if (k0 + rw >= w.Nk || c >= w.d || (redo >> rw & 1)) continue;
+        if (k0 + rw >= w.Nk || c >= w.d) continue;
         f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int x = 0; x < 4; ++x) sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * WAVE_B) + which * 32 * C + sum_at<C>(rw, col));
@@ -1108,6 +1134,15 @@ window_bwd_dkv_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, co
             for (int j = 0; j < 4; ++j) y[j] = (T)sum[j];
             *reinterpret_cast<vec4*>((which ? dVg : dKg) + ((int64_t)bg * w.Nk + k0 + rw) * w.d + c) = y;
         }
+    }
+    if (redo != 0) {                                        // (window_attn_exact.h)
+        const KeyOut<T> to{dKg + ((int64_t)bg * w.Nk + k0) * w.d, dVg + ((int64_t)bg * w.Nk + k0) * w.d,
+                           split && ns > 1 ? parts + ((int64_t)(bg * nsb + kblk) * ns + part) * 2 * 32 * w.d : nullptr,
+                           split && ns > 1 ? parts + (((int64_t)(bg * nsb + kblk) * ns + part) * 2 + 1) * 32 * w.d : nullptr};
+        stored();
+        __syncthreads();
+        exact_keys<T, D>(redo, 4, wave, k0, 0, w, b, kvh, len, pa, pz, j0, j1, nt, tq0, BQ, Qg, Kg, Vg, dOg, st, nqp, rows, to, col0, min(w.d, col0 + C),
+                         lane);
     }
 }
 

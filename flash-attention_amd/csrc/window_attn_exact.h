@@ -1,11 +1,13 @@
 // The way out for rows whose tiles hold infinities or NaN that the rows themselves do not see.
 //
 // In the tiled kernels a hidden pair has weight 0, and 0 times a NaN or an infinity is NaN: a value that one row
-// sees would reach the others of its tile.  Nothing in the loops looks for that; at the end a row whose float32 sums
-// are not finite although its statistics are is computed again here, key by key (or query by query) over what it
-// sees and nothing else, by one wave with the columns on its lanes.  Slow (about a microsecond per two keys), taken
-// only when such values are there; a row whose statistics are NaN is NaN by definition and is left.  The looks themselves
-// (a ballot per 32 rows, once) cost nothing that shows: 452 us for 16 heads of 16384 positions with a window of 4096, with and without.
+// sees would reach the others of its tile.  Nothing in the loops looks for that.  Where at the end a wave's float32 sums
+// are not finite, it looks through what its tiles held hidden (the tiles at the edges of what its rows see, no more) for
+// columns that are not finite; in those alone its rows are formed again, key by key (or its keys query by query) over
+// what they see and nothing else, with the columns on the lanes and until nothing finite is left in them.
+// In the ordinary case it is a ballot per 32 rows, which costs nothing that shows: 452 us for 16 heads of 16384 positions with
+// a window of 4096, with and without.  There, a value row of infinities halfway takes the forward to 22 ms and the backward to
+// 176 (one wave forms 32 rows of 4096 keys); one that every later row sees costs the look, 0.7 and 9.5 ms.
 #ifndef MYFA_WINDOW_ATTN_EXACT_H_
 #define MYFA_WINDOW_ATTN_EXACT_H_
 #include "window_attn_common.h"
@@ -25,16 +27,7 @@ __device__ __forceinline__ uint32_t not_finite_rows(const f32x16 (&acc)[NDB], bo
     return (uint32_t)(b | b >> 32);
 }
 __device__ __forceinline__ bool finite(float x) { return x - x == 0.f; }
-template <typename T, int KS, typename Frag> __device__ __forceinline__ bool finite_chunks(const Frag (&f)[KS]) {
-    constexpr int EPC = 16 / (int)sizeof(T);
-    typedef T vec __attribute__((ext_vector_type(EPC)));
-    float x = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int j = 0; j < EPC; ++j) x = __builtin_fmaf((float)__builtin_bit_cast(vec, f[ks])[j], 0.f, x);
-    return x == 0.f;
-}
+__device__ __forceinline__ bool any_lane(bool x) { return __builtin_amdgcn_ballot_w64(x) != 0; }
 
 template <typename T, int D> struct LaneRow {
     static constexpr int N = D / 64;
@@ -45,7 +38,10 @@ template <typename T, int D> struct LaneRow {
     }
     __device__ __forceinline__ LaneRow(const T* p, int d, int lane) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = 64 * i + lane < d ? (float)p[64 * i + lane] : 0.f;
+        for (int i = 0; i < N; ++i) {                 // (no branch around the load: one would wait for it there)
+            const float y = (float)p[min(64 * i + lane, d - 1)];
+            x[i] = 64 * i + lane < d ? y : 0.f;
+        }
     }
     __device__ __forceinline__ float dot(const LaneRow& y) const {
         float s = 0.f;
@@ -61,55 +57,120 @@ template <typename T, int D> struct LaneRow {
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] *= f;
     }
-    // columns [c0, c1)
-    template <typename O> __device__ __forceinline__ void store(O* p, float f, int c0, int c1, int lane) const {
+    // bit i: column 64 i + lane
+    static __device__ __forceinline__ uint32_t all(int d, int lane) {
+        uint32_t cols = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) cols |= (uint32_t)(64 * i + lane < d) << i;
+        return cols;
+    }
+    __device__ __forceinline__ uint32_t not_finite() const {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) bad |= (uint32_t)!finite(x[i]) << i;
+        return bad;
+    }
+    // the columns of `cols` within [c0, c1)
+    template <typename O> __device__ __forceinline__ void store(O* p, float f, uint32_t cols, int c0, int c1, int lane) const {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (64 * i + lane >= c0 && 64 * i + lane < c1) p[64 * i + lane] = (O)(x[i] * f);
+            if ((cols >> i & 1) && 64 * i + lane >= c0 && 64 * i + lane < c1) p[64 * i + lane] = (O)(x[i] * f);
     }
 };
 
-// f(key) over the keys that position p sees
-template <class F> __device__ __forceinline__ void for_seen_keys(const WindowShape& w, int p, F&& f) {
-    const int lo = max(0, p - w.window + 1);
-    for (int j = 0; j < min(w.sinks, lo); ++j) f(j);
-    for (int j = lo; j <= p; ++j) f(j);
+// Columns that are not finite in keys of `base` which the wave with rows at positions p0 .. p0 + 31 goes through and some
+// of these rows do not see.
+template <typename T, int D, int BN>
+__device__ __forceinline__ uint32_t hidden_keys(const KeyTiles<BN>& kt, const WindowShape& w, int p0, const T* base, int64_t stride, int lane) {
+    uint32_t bad = 0;
+    for (int t = 0; t < kt.ntiles; ++t) {
+        const int k0 = kt.first_key(t);
+        if (k0 > p0 + 31 || (k0 + BN <= p0 - w.window + 1 && k0 >= w.sinks)) continue;                          // nothing of it is seen
+        if (k0 + BN - 1 <= p0 && (k0 > p0 + 31 - w.window || k0 + BN <= w.sinks)) continue;                     // all of it is
+        for (int key = k0; key < k0 + BN; ++key)
+            if (kt.one(key, w.sinks)) bad |= LaneRow<T, D>(base + key * stride, w.d, lane).not_finite();
+    }
+    return bad;
 }
 
+constexpr int kAtOnce = 4;             // rows of an exact sum whose loads and reductions overlap
+
+// f(key, n): keys key .. key + n - 1, over the keys that position p sees, while it returns true
+template <class F> __device__ __forceinline__ void for_seen_keys(const WindowShape& w, int p, F&& f) {
+    const int lo = max(0, p - w.window + 1), sinks = min(w.sinks, lo);
+    for (int j = 0; j < sinks; j += kAtOnce)
+        if (!f(j, min(kAtOnce, sinks - j))) return;
+    for (int j = lo; j <= p; j += kAtOnce)
+        if (!f(j, min(kAtOnce, p + 1 - j))) return;
+}
+
+// What has been stored is stored: nothing of the wave's comes after what it stores next.
+__device__ __forceinline__ void stored() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 template <typename T, int D>
-__device__ __forceinline__ void exact_fwd_row(const T* q, const T* Kh, const T* Vh, T* out, const WindowShape& w, int p, int lane) {
+__device__ __forceinline__ void exact_fwd_row(const T* q, const T* Kh, const T* Vh, T* out, const WindowShape& w, int p, uint32_t cols, int lane) {
     using L = LaneRow<T, D>;
     const L qr(q, w.d, lane);
     L o;
     float m = -INFINITY, l = 0.f;
-    for_seen_keys(w, p, [&](int j) {
-        const float s = qr.dot(L(Kh + j * w.ks[2], w.d, lane)) * (w.scale * kLog2eW);
-        const float m_new = fmaxf(m, s), ref = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = __builtin_amdgcn_exp2f(m - ref), pj = __builtin_amdgcn_exp2f(s - ref);
+    for_seen_keys(w, p, [&](int j, int n) {
+        float s[kAtOnce], m_new = m;
+        L v[kAtOnce];
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x) {
+            const int key = j + min(x, n - 1);
+            s[x] = qr.dot(L(Kh + key * w.ks[2], w.d, lane)) * (w.scale * kLog2eW);
+            v[x] = L(Vh + key * w.vs[2], w.d, lane);
+            m_new = fmaxf(m_new, s[x]);
+        }
+        const float ref = m_new == -INFINITY ? 0.f : m_new, alpha = __builtin_amdgcn_exp2f(m - ref);
         if (m_new > m) o.scale(alpha);
-        l = l * alpha + pj;
+        l *= alpha;
         m = m_new;
-        o.add(pj, L(Vh + j * w.vs[2], w.d, lane));
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x)
+            if (x < n) {
+                const float pj = __builtin_amdgcn_exp2f(s[x] - ref);
+                l += pj;
+                o.add(pj, v[x]);
+            }
+        return any_lane((cols & ~o.not_finite()) != 0);
     });
-    o.store(out, 1.f / l, 0, w.d, lane);
+    o.store(out, 1.f / l, cols, 0, w.d, lane);
 }
 
 template <typename T, int D>
 __device__ __forceinline__ void exact_dq_row(const T* q, const T* dout, const T* Kh, const T* Vh, float lse2, float ndelta, T* out,
-                                             const WindowShape& w, int p, int lane) {
+                                             const WindowShape& w, int p, uint32_t cols, int lane) {
     using L = LaneRow<T, D>;
     const L qr(q, w.d, lane), dr(dout, w.d, lane);
     L dq;
-    for_seen_keys(w, p, [&](int j) {
-        const L k(Kh + j * w.ks[2], w.d, lane);
-        const float pj = __builtin_amdgcn_exp2f(__builtin_fmaf(qr.dot(k), w.scale * kLog2eW, -lse2));
-        dq.add(pj * (dr.dot(L(Vh + j * w.vs[2], w.d, lane)) + ndelta), k);
+    for_seen_keys(w, p, [&](int j, int n) {
+        float ds[kAtOnce];
+        L k[kAtOnce];
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x) {
+            const int key = j + min(x, n - 1);
+            k[x] = L(Kh + key * w.ks[2], w.d, lane);
+            const float pj = __builtin_amdgcn_exp2f(__builtin_fmaf(qr.dot(k[x]), w.scale * kLog2eW, -lse2));
+            ds[x] = pj * (dr.dot(L(Vh + key * w.vs[2], w.d, lane)) + ndelta);
+        }
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x)
+            if (x < n) dq.add(ds[x], k[x]);
+        return any_lane((cols & ~dq.not_finite()) != 0);
     });
-    dq.store(out, w.scale, 0, w.d, lane);
+    dq.store(out, w.scale, cols, 0, w.d, lane);
 }
 
-// dK and dV of a key: f_query(add) calls add(q row, dout row, lse2, -delta) for every query of the workgroup's tiles that
-// sees the key.
+// Columns of dQ that hidden keys reach: a value that is not finite makes the hidden dS NaN, and with it every column.
+template <typename T, int D, int BN>
+__device__ __forceinline__ uint32_t hidden_for_dq(const KeyTiles<BN>& kt, const WindowShape& w, int p0, const T* Kh, const T* Vh, int lane) {
+    if (any_lane(hidden_keys<T, D>(kt, w, p0, Vh, w.vs[2], lane) != 0)) return LaneRow<T, D>::all(w.d, lane);
+    return hidden_keys<T, D>(kt, w, p0, Kh, w.ks[2], lane);
+}
+
+// dK and dV of a key, a few queries at a time: rows q + x qs, dout + x d, statistics lse2[x], ndelta[x] for x < n
 template <typename T, int D> struct ExactKey {
     using L = LaneRow<T, D>;
     L k, v, dk, dv;
@@ -117,11 +178,23 @@ template <typename T, int D> struct ExactKey {
     int d, lane;
     __device__ __forceinline__ ExactKey(const T* kr, const T* vr, const WindowShape& w, int ln)
         : k(kr, w.d, ln), v(vr, w.d, ln), sl2(w.scale * kLog2eW), d(w.d), lane(ln) {}
-    __device__ __forceinline__ void add(const T* q, const T* dout, float lse2, float ndelta) {
-        const L qr(q, d, lane), dr(dout, d, lane);
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(qr.dot(k), sl2, -lse2));
-        dv.add(p, dr);
-        dk.add(p * (dr.dot(v) + ndelta), qr);
+    __device__ __forceinline__ void add(const T* q, int64_t qs, const T* dout, const float* lse2, const float* ndelta, int n) {
+        float p[kAtOnce], ds[kAtOnce];
+        L qr[kAtOnce], dr[kAtOnce];
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x) {
+            const int i = min(x, n - 1);
+            qr[x] = L(q + i * qs, d, lane);
+            dr[x] = L(dout + (int64_t)i * d, d, lane);
+            p[x] = __builtin_amdgcn_exp2f(__builtin_fmaf(qr[x].dot(k), sl2, -lse2[i]));
+            ds[x] = p[x] * (dr[x].dot(v) + ndelta[i]);
+        }
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x)
+            if (x < n) {
+                dv.add(p[x], dr[x]);
+                dk.add(ds[x], qr[x]);
+            }
     }
 };
 

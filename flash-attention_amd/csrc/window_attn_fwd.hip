@@ -130,12 +130,7 @@ window_attn_fwd_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
 
     // lane (r, h) holds columns 32 db + 8 g + 4 h + 0..3 of its query in registers 4g..4g+3 of block db
     const float total = half_exchange_sum(l);
-    // (window_attn_exact.h)
     const uint32_t redo = not_finite_rows(o, live && finite(total));
-    for (uint32_t left = redo; left != 0; left &= left - 1) {
-        const int x = q0 + 32 * wave + __builtin_ctz(left);
-        exact_fwd_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + x * w.qs[2], Kh, Vh, Og + ((int64_t)bh * w.Nq + x) * w.d, w, x + kt.shift, lane);
-    }
     if (qrow < w.Nq) {
         const float inv = live ? 1.0f / total : 0.f;
         T* orow = Og + ((int64_t)bh * w.Nq + qrow) * w.d;
@@ -148,10 +143,18 @@ window_attn_fwd_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
                 vec4 x;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = live ? (T)(o[db][4 * g + j] * inv) : (T)0.f;
-                if (c < w.d && !(redo >> r & 1)) *reinterpret_cast<vec4*>(orow + c) = x;
+                if (c < w.d) *reinterpret_cast<vec4*>(orow + c) = x;
             }
         if (LSEg != nullptr && h == 0)
             LSEg[(int64_t)bh * w.Nq + qrow] = live ? (m + __builtin_amdgcn_logf(total)) * kLn2W : -INFINITY;
+    }
+    if (redo != 0) {                                        // (window_attn_exact.h)
+        const uint32_t cols = hidden_keys<T, D>(kt, w, q0 + 32 * wave + kt.shift, Vh, w.vs[2], lane);
+        stored();
+        for (uint32_t left = any_lane(cols != 0) ? redo : 0; left != 0; left &= left - 1) {
+            const int x = q0 + 32 * wave + __builtin_ctz(left);
+            exact_fwd_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + x * w.qs[2], Kh, Vh, Og + ((int64_t)bh * w.Nq + x) * w.d, w, x + kt.shift, cols, lane);
+        }
     }
 }
 
@@ -334,12 +337,7 @@ window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
     masked_tiles(min(first_after, ntiles), ntiles);
 
     const float total = half_exchange_sum(l);
-    // (window_attn_exact.h)
     const uint32_t redo = not_finite_rows(o, live && finite(total));
-    for (uint32_t left = redo; left != 0; left &= left - 1) {
-        const int x = q0 + 32 * wave + __builtin_ctz(left);
-        exact_fwd_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + x * w.qs[2], Kh, Vh, Og + ((int64_t)bh * w.Nq + x) * w.d, w, x + kt.shift, lane);
-    }
     if (qrow < w.Nq) {
         const float inv = live ? 1.0f / total : 0.f;
         T* orow = Og + ((int64_t)bh * w.Nq + qrow) * w.d;
@@ -351,10 +349,18 @@ window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
                 typename M::vec4 x;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = live ? (T)(o[db][4 * g + j] * inv) : (T)0.f;
-                if (c < w.d && !(redo >> r & 1)) *reinterpret_cast<typename M::vec4*>(orow + c) = x;
+                if (c < w.d) *reinterpret_cast<typename M::vec4*>(orow + c) = x;
             }
         if (LSEg != nullptr && h == 0)
             LSEg[(int64_t)bh * w.Nq + qrow] = live ? (m + __builtin_amdgcn_logf(total)) * kLn2W : -INFINITY;
+    }
+    if (redo != 0) {                                        // (window_attn_exact.h)
+        const uint32_t cols = hidden_keys<T, D>(kt, w, q0 + 32 * wave + kt.shift, Vh, w.vs[2], lane);
+        stored();
+        for (uint32_t left = any_lane(cols != 0) ? redo : 0; left != 0; left &= left - 1) {
+            const int x = q0 + 32 * wave + __builtin_ctz(left);
+            exact_fwd_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + x * w.qs[2], Kh, Vh, Og + ((int64_t)bh * w.Nq + x) * w.d, w, x + kt.shift, cols, lane);
+        }
     }
 }
 
@@ -457,13 +463,7 @@ window_attn_fwd_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, c
         if (lane == 0) redo_of[wave] = bad;
     }
     __syncthreads();
-    const uint32_t redo = __builtin_amdgcn_readfirstlane(redo_of[0] | redo_of[1] | redo_of[2] | redo_of[3]);      // (window_attn_exact.h)
-    int turn = 0;
-    for (uint32_t left = redo; left != 0; left &= left - 1, ++turn) {
-        if ((turn & 3) != wave) continue;
-        const int x = q0 + __builtin_ctz(left);
-        exact_fwd_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + x * w.qs[2], Kh, Vh, Og + ((int64_t)bh * w.Nq + x) * w.d, w, x + kt.shift, lane);
-    }
+    const uint32_t redo = __builtin_amdgcn_readfirstlane(redo_of[0] | redo_of[1] | redo_of[2] | redo_of[3]);
     typedef T vec4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int e = tid; e < 32 * D / 4; e += 256) {
@@ -487,8 +487,19 @@ window_attn_fwd_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, c
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = sees_any ? (T)(sum[j] * inv) : (T)0.f;
         const int64_t at = (int64_t)bh * w.Nq + q0 + row;
-        if (col < w.d && !(redo >> row & 1)) *reinterpret_cast<vec4*>(Og + at * w.d + col) = y;
+        if (col < w.d) *reinterpret_cast<vec4*>(Og + at * w.d + col) = y;
         if (col == 0 && LSEg != nullptr) LSEg[at] = sees_any ? (top + __builtin_amdgcn_logf(total)) * kLn2W : -INFINITY;
+    }
+    if (redo != 0) {                                        // (window_attn_exact.h)
+        const uint32_t cols = hidden_keys<T, D>(kt, w, q0 + kt.shift, Vh, w.vs[2], lane);
+        stored();
+        __syncthreads();
+        int turn = 0;
+        for (uint32_t left = any_lane(cols != 0) ? redo : 0; left != 0; left &= left - 1, ++turn) {
+            if ((turn & 3) != wave) continue;
+            const int x = q0 + __builtin_ctz(left);
+            exact_fwd_row<T, D>(Qg + b * w.qs[0] + head * w.qs[1] + x * w.qs[2], Kh, Vh, Og + ((int64_t)bh * w.Nq + x) * w.d, w, x + kt.shift, cols, lane);
+        }
     }
 }
 

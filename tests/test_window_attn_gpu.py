@@ -198,6 +198,43 @@ def test_what_a_row_does_not_see_may_hold_anything(mfa, shape, what):
     assert torch.isnan(got["dq"][:, :, row_bad.cuda()]).any(-1).all()
 
 
+@pytest.mark.parametrize("shape", [(1, 4, 2, 260, 260, 64, 20, 3, BF16), (1, 2, 1, 200, 200, 128, 20, 2, F32), (1, 2, 1, 180, 180, 256, 20, 2, F16),     # few rows
+                                   (1, 100, 100, 260, 260, 128, 20, 3, F16), (1, 100, 100, 200, 200, 160, 20, 2, BF16), (1, 100, 100, 200, 200, 96, 20, 2, F32)],
+                         ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+def test_a_column_that_is_not_finite(mfa, shape):
+    """One column of a value, and of an output gradient, in a place that some rows of a tile see: the others keep theirs, and what does
+    not depend on it keeps all."""
+    B, H, G, nq, nk, d, window, sinks, dtype = shape
+    q, k, v, dout = _inputs(B, H, G, nq, nk, d, dtype, 5)
+    vis = _visible(B, nq, nk, window, sinks, None)
+    want = ref.attention(q, k, v, vis, 0.125, dtype, dout)
+    at, col = 141, 37
+    others = torch.arange(d) != col
+
+    def rows(t, keep):
+        return t[:, :, keep.to(t.device)]
+    v_bad = v.clone()
+    v_bad[:, :, at, col] = float("inf")
+    sees = vis[0][:, at]
+    touched = vis[0][sees].any(0)                              # keys that share a row with it
+    got = _run(mfa, *(t.cuda() for t in (q, k, v_bad, dout)), window, sinks, 0.125, None)
+    ref.check("out", got["out"][..., others.cuda()], tuple(t.expand_as(want["out"][0])[..., others] for t in want["out"]))
+    ref.check("out", rows(got["out"], ~sees), tuple(rows(t, ~sees) for t in want["out"]))
+    ref.check("dq", rows(got["dq"], ~sees), tuple(rows(t, ~sees) for t in want["dq"]))
+    ref.check("dk", rows(got["dk"], ~touched), tuple(rows(t, ~touched) for t in want["dk"]))
+    ref.check("dv", got["dv"], want["dv"])
+    assert not torch.isfinite(rows(got["out"], sees)[..., col]).any()
+    d_bad = dout.clone()
+    d_bad[:, :, at, col] = float("nan")
+    touched = vis[0][at]
+    got = _run(mfa, *(t.cuda() for t in (q, k, v, d_bad)), window, sinks, 0.125, None)
+    keep = torch.arange(nq) != at
+    ref.check("dq", rows(got["dq"], keep), tuple(rows(t, keep) for t in want["dq"]))
+    ref.check("dk", rows(got["dk"], ~touched), tuple(rows(t, ~touched) for t in want["dk"]))
+    ref.check("dv", got["dv"][..., others.cuda()], tuple(t.expand_as(want["dv"][0])[..., others] for t in want["dv"]))
+    ref.check("dv", rows(got["dv"], ~touched), tuple(rows(t, ~touched) for t in want["dv"]))
+
+
 def test_strided_views(mfa):
     """(B, N, H, d) layouts and slices of one fused projection give what dense copies give, bit for bit."""
     torch.manual_seed(0)
