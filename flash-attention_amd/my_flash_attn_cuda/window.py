@@ -29,5 +29,8 @@ def window_attn_bwd(dout, q, k, v, out, lse, window, sinks=0, scale=1.0, seq_len
 
 
 def window_attn_func(q, k, v, window, sinks=0, scale=1.0, seq_lens=None):
-    """window_attn_fwd with autograd support (once differentiable), for everything it serves."""
+    """window_attn_fwd with autograd support (once differentiable), for everything it serves.
+
+    Capturing a training step into a graph: take the gradients with torch.autograd.grad, or let no autograd graph
+    of the same leaves that was built outside live on (torch accumulates into a leaf on the stream it was first used on)."""
     return _host.window_attn_func(q, k, v, window, sinks, scale, seq_lens)

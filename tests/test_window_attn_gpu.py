@@ -353,6 +353,36 @@ def test_graph_replays(mfa):
             assert torch.equal(a, b)
 
 
+def test_captured_training_step(mfa):
+    """Forward and gradients through autograd, captured; the workspace is the graph's own, whatever eager calls do in between."""
+    leaves = [t.cuda().requires_grad_() for t in _inputs(2, 4, 2, 300, 300, 64, BF16, 9)[:3]]
+    dout = _inputs(2, 4, 2, 300, 300, 64, BF16, 9)[3].cuda()
+
+    def step(x):
+        out = mfa.window_attn_func(*x, 40, sinks=4, scale=0.125)
+        return (out.detach(), *torch.autograd.grad(out, x, dout))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    graph, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(leaves)
+    with torch.cuda.graph(second):
+        held2 = step(leaves)
+    for seed in range(3):
+        with torch.no_grad():
+            for t, x in zip(leaves, _inputs(2, 4, 2, 300, 300, 64, BF16, 20 + seed)):
+                t.copy_(x)
+        graph.replay()
+        second.replay()
+        want = step([t.detach().clone().requires_grad_() for t in leaves])
+        torch.cuda.synchronize()
+        for a, b, c in zip(held, held2, want):
+            assert torch.equal(a, c) and torch.equal(b, c)
+
+
 def test_refusals(mfa):
     q, k, v, dout = (t.cuda() for t in _inputs(1, 4, 2, 32, 48, 64, BF16, 0))
     lens = torch.tensor([48], dtype=torch.int32, device="cuda")
