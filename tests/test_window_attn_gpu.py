@@ -253,6 +253,23 @@ def test_strided_views(mfa):
         assert torch.equal(a[name], b[name]), name
 
 
+def test_strides_beyond_32_bits(mfa):
+    """Batches that lie more than 2^32 bytes apart."""
+    dense = [t.cuda() for t in _inputs(2, 4, 2, 150, 150, 64, BF16, 3)]
+    apart = (1 << 31) + 64
+    pool = torch.empty(apart + 3 * 4 * 150 * 64, dtype=BF16, device="cuda")
+    far, at = [], 0
+    for t in dense[:3]:
+        H = t.shape[1]
+        x = pool.as_strided(t.shape, (apart, 150 * 64, 64, 1), at)
+        x.copy_(t)
+        far.append(x)
+        at += H * 150 * 64
+    want, got = _run(mfa, *dense, 30, 3, 0.125, None), _run(mfa, *far, dense[3], 30, 3, 0.125, None)
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+
+
 def test_same_result_every_time(mfa):
     q, k, v, dout = (t.cuda() for t in _inputs(2, 8, 2, 700, 700, 128, BF16, 4))
     first = _run(mfa, q, k, v, dout, 128, 4, 0.1, [700, 600])
