@@ -53,7 +53,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* waves, uint
 template <int PER>
 __global__ void __launch_bounds__(kSelThreads)
 paged_evict_select_kernel(EvictShape e) {
-    __shared__ uint32_t hist[kBins], waves[kSelWaves], found[2];
+    __shared__ uint32_t hist[kBins], waves[kSelWaves], found[3];
     const int bg = blockIdx.x, b = bg / e.Hkv, tid = threadIdx.x;
     const int len = min(max(e.lens[b], 0), e.cap), keep = min(len, e.budget);
     const float* sums = e.sums + (int64_t)bg * e.cap;
@@ -108,11 +108,18 @@ paged_evict_select_kernel(EvictShape e) {
                 const bool second = before + c0 < quota;
                 found[0] = (uint32_t)(second ? hi - 1 : hi);
                 found[1] = quota - before - (second ? c0 : 0u);
+                found[2] = second ? c1 : c0;
             }
             __syncthreads();
             limit = (above << bits) | found[0];
             quota = found[1];
+            const bool whole = quota == found[2];                      // the digit's keys are all among them: no more digits
             __syncthreads();
+            if (whole) {                                               // (the least key is -infinity's 0x007FFFFF: no wrap)
+                limit = (limit << shift) - 1;
+                quota = 0;
+                break;
+            }
         }
     }
     const bool none = !all && e.budget - e.sinks - e.recent == 0;
