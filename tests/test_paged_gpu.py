@@ -305,6 +305,38 @@ def test_evict_bad_pages(mfa):
     assert torch.equal(k_pool[same].nan_to_num(9.0), before[same].nan_to_num(9.0))
 
 
+@pytest.mark.parametrize("case", [([5000, 40, 300], 2, 16, 16, 300, 4, 20), ([2048, 2049], 1, 16, 128, 128, 0, 0), ([2049], 1, 16, 128, 129, 1, 1),
+                                  ([1000], 1, 10, 64, 256, 4, 32), ([1000], 1, 10, 64, 257, 4, 32)], ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+@pytest.mark.parametrize("kind", ["plain", "ties"])
+def test_evict_around_one_launch(mfa, case, kind):
+    """Sizes on both sides of what the selection moves by itself."""
+    test_evict(mfa, case, kind)
+
+
+def test_evict_bad_pages_of_many_keys(mfa):
+    """The same as test_evict_bad_pages where a second launch moves the keys."""
+    c = Cache([640, 640], 1, 16, 128, BF16, 11, spare=40)
+    k_pool, v_pool, table, L = c.gpu()
+    new = [[c.free.pop() for _ in range(20)] for _ in range(2)]
+    new[0][7] = c.pages + 3
+    new_table = torch.tensor(new, dtype=torch.int32, device="cuda")
+    table[1, 2] = -7
+    before = k_pool.clone()
+    mfa.paged_kv_evict(k_pool, v_pool, torch.zeros(2, 1, 640, device="cuda"), table, L, new_table, 320, sinks=160, recent=160)
+    same = torch.ones(c.pages, dtype=torch.bool, device="cuda")
+    for b in range(2):
+        for i in range(20):
+            if (b, i) == (0, 7):
+                continue
+            at = 16 * i if i < 10 else 640 - 320 + 16 * i
+            same[new[b][i]] = False
+            if (b, i) == (1, 2):
+                assert torch.isnan(k_pool[new[b][i]]).all() and torch.isnan(v_pool[new[b][i]]).all()
+            else:
+                assert torch.equal(k_pool[new[b][i]].cpu()[0], c.k[b][0, at:at + 16]) and torch.equal(v_pool[new[b][i]].cpu()[0], c.v[b][0, at:at + 16])
+    assert torch.equal(k_pool[same].nan_to_num(9.0), before[same].nan_to_num(9.0))
+
+
 def test_prefill_append_decode_evict(mfa):
     """A padded batch of prompts through window attention into the cache, tokens decoded with the same window, the
     cache cut by the weights, and decoding on: every step against the definition on the keys it should see."""
