@@ -322,10 +322,11 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
             });
             finish(1);
             add(IC<1>{}, [&](auto ic) __attribute__((always_inline)) {
-                if constexpr (decltype(ic)::value == (2 * DB > FW ? 2 * DB - FW : 0)) behind();
+                constexpr int from = 2 * DB > FW ? 2 * DB - FW : 0;              // behind the last transposing read
+                if constexpr (decltype(ic)::value >= from) behind(IC<decltype(ic)::value - from>{});
             });
         } else {
-            behind();
+            behind(IC<0>{});
         }
         const int was = cur;
         cur = nxt; nxt = fre; fre = was;
@@ -334,7 +335,7 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
         for (int t = t0; t < t1; ++t) {
             const int k0 = kt.first_key(t);
             tile(t, k0, !(k0 > wave_hi || (k0 + BN <= wave_lo - w.window + 1 && k0 >= w.sinks)), IC<1>{},
-                 [&]() __attribute__((always_inline)) { fetch(t + 2, fre); });
+                 [&](auto ic) __attribute__((always_inline)) { if constexpr (decltype(ic)::value == 0) fetch(t + 2, fre); });
         }
     };
     const int f0 = kt.whole_from(w.window, 128), f1 = kt.whole_to(128);      // tiles that all rows see whole
@@ -343,18 +344,27 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
         const T* kp = Kh + (int64_t)kt.first_key(f0 + 2) * w.ks[2];
         const T* vp = Vh + (int64_t)kt.first_key(f0 + 2) * w.vs[2];
         const int64_t kstep = BN * w.ks[2], vstep = BN * w.vs[2];
-        for (int t = f0; t < f1; ++t) {
-            tile(t, 0, true, IC<0>{}, [&]() __attribute__((always_inline)) {
-                if (t + 2 < f1) {
-                    kfetch.fetch(kp, lds + fre * TILE_B, true, [](int) { return true; });
-                    vfetch.fetch(vp, lds + (3 + (t & 1)) * TILE_B, true, [](int) { return true; });
-                } else {
-                    fetch(t + 2, fre);
-                }
-            });
-            kp += kstep;
-            vp += vstep;
-        }
+        // (pieces: tile t + 2 is whole too, and is requested two pieces at a step)
+        auto whole_tiles = [&](int t0, int t1, auto pieces) __attribute__((always_inline)) {
+            for (int t = t0; t < t1; ++t) {
+                tile(t, 0, true, IC<0>{}, [&](auto ic) __attribute__((always_inline)) {
+                    constexpr int i = decltype(ic)::value, LPT = TileFetch<T, D, BN, 256>::LPT;
+                    static_assert(LPT <= (2 * DB < FW ? 2 * DB : FW), "two pieces a step");
+                    if constexpr (decltype(pieces)::value) {
+                        if constexpr (i < LPT) {
+                            kfetch.template piece<i>(kp, lds + fre * TILE_B);
+                            vfetch.template piece<i>(vp, lds + (3 + (t & 1)) * TILE_B);
+                        }
+                    } else if constexpr (i == 0) {
+                        fetch(t + 2, fre);
+                    }
+                });
+                kp += kstep;
+                vp += vstep;
+            }
+        };
+        whole_tiles(f0, f1 - 2, IC<1>{});
+        whole_tiles(max(f0, f1 - 2), f1, IC<0>{});
     }
     masked_tiles(min(max(f0, f1), ntiles), ntiles);
 

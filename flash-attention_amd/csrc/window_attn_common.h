@@ -134,6 +134,14 @@ template <typename T, int D, int ROWS, int THREADS> struct TileFetch {
             off[i] = ch * (16 / (int)sizeof(T)) < d ? (row[i] * (int)row_stride + ch * (16 / (int)sizeof(T))) * (int)sizeof(T) : kOffPast;
         }
     }
+    // piece I of a whole tile: an LDS-DMA instruction takes its wave about 40 cycles to issue, so that pieces dealt one
+    // to an MFMA are hidden and several in a row are not
+    template <int I> __device__ __forceinline__ void piece(const T* base, char* lds) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, kTileBytesMax, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(lds + 1024 * (wave * LPT + I)), 16, off[I], 0, 0, 0);
+#endif
+    }
     // rows of the tile for which keep(row) does not hold read as zeros
     template <class Keep>
     __device__ __forceinline__ void fetch(const T* base, char* lds, bool all, Keep&& keep) const {

@@ -170,10 +170,11 @@ window_attn_fwd_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
 //   rescale of O, 64 multiplications a lane, is in most tiles.
 //   The tiles that every row of the workgroup sees whole run in a loop without masks, bounds or tile arithmetic.
 // Measured (bf16, d 128): 16 heads of 16384 positions, window 4096: 452 us, 1065 TFLOP/s of what is seen, where a
-// library product of 8192^3 reaches 1194; B 4, 32 heads of 4096 positions, window 1024: 295 us, 817 (a tenth of the work
+// library product of 8192^3 reaches 1194; B 4, 32 heads of 4096 positions, window 1024: 290 us, 832 (a tenth of the work
 // is in tiles that the masks halve).  Bound by the matrix pipe at the clock that the power limit leaves it: on operands
-// that are all ones the first takes 358 us.  Forming each half of a tile's weights beside the products of the other
-// half changed neither (460 against 459 us, all ones 360 against 358): the two workgroups of a CU do that already.
+// that are all ones the first takes 335 us.  With the next tiles' requests in a row instead of one to a step: 490 against 478
+// us on one card, all ones 358 against 335.  Forming each half of a tile's weights beside the products of the other half: no
+// faster (458 against 453, all ones 339 against 334), the two workgroups of a CU do that already.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 2)
 window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T* __restrict__ Vg,
@@ -286,7 +287,7 @@ window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
                                o[i % DB] = M::run(a, pb[i / DB], o[i % DB]);
                            },
                            [&](auto ic) __attribute__((always_inline)) {
-                               if constexpr (decltype(ic)::value == NP - FW) behind();
+                               if constexpr (decltype(ic)::value >= NP - FW) behind(IC<decltype(ic)::value - (NP - FW)>{});
                            });
     };
     tile_ready();
@@ -304,8 +305,9 @@ window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
                 softmax(s);
             }
             tile_ready();
-            if (some) add_pv(lds + (2 + (t & 1)) * TILE_B, [&]() __attribute__((always_inline)) { fetch_v(t + 1); fetch_k(t + 2); });
-            else { fetch_v(t + 1); fetch_k(t + 2); }
+            auto ahead = [&](auto ic) __attribute__((always_inline)) { if constexpr (decltype(ic)::value == 0) { fetch_v(t + 1); fetch_k(t + 2); } };
+            if (some) add_pv(lds + (2 + (t & 1)) * TILE_B, ahead);
+            else ahead(IC<0>{});
         }
     };
     masked_tiles(0, min(f0, ntiles));
@@ -315,24 +317,31 @@ window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
         const T* vp = Vh + (int64_t)kt.first_key(f0 + 1) * w.vs[2];
         const int64_t kstep = BN * w.ks[2], vstep = BN * w.vs[2];
         int buf = f0 & 1;
-        for (int t = f0; t < f1; ++t) {
-            f32x16 s[2];
-            logits(lds + buf * TILE_B, s);
-            softmax(s);
-            tile_ready();
-            add_pv(lds + (2 + buf) * TILE_B, [&]() __attribute__((always_inline)) {
-                if (t + 2 < f1) {
-                    vfetch.fetch(vp, lds + (3 - buf) * TILE_B, true, [](int) { return true; });
-                    kfetch.fetch(kp, lds + buf * TILE_B, true, [](int) { return true; });
-                } else {
-                    fetch_v(t + 1);
-                    fetch_k(t + 2);
-                }
-            });
-            kp += kstep;
-            vp += vstep;
-            buf ^= 1;
-        }
+        // (pieces: tiles t + 1 and t + 2 are whole too, and are requested a piece at a step)
+        auto whole_tiles = [&](int t0, int t1, auto pieces) __attribute__((always_inline)) {
+            for (int t = t0; t < t1; ++t) {
+                f32x16 s[2];
+                logits(lds + buf * TILE_B, s);
+                softmax(s);
+                tile_ready();
+                add_pv(lds + (2 + buf) * TILE_B, [&](auto ic) __attribute__((always_inline)) {
+                    constexpr int i = decltype(ic)::value, LPT = TileFetch<T, D, BN, 256>::LPT;
+                    static_assert(2 * LPT <= FW, "a piece a step");
+                    if constexpr (decltype(pieces)::value) {
+                        if constexpr (i < LPT) vfetch.template piece<i>(vp, lds + (3 - buf) * TILE_B);
+                        else if constexpr (i < 2 * LPT) kfetch.template piece<i - LPT>(kp, lds + buf * TILE_B);
+                    } else if constexpr (i == 0) {
+                        fetch_v(t + 1);
+                        fetch_k(t + 2);
+                    }
+                });
+                kp += kstep;
+                vp += vstep;
+                buf ^= 1;
+            }
+        };
+        whole_tiles(f0, f1 - 2, IC<1>{});
+        whole_tiles(max(f0, f1 - 2), f1, IC<0>{});
     }
     masked_tiles(min(first_after, ntiles), ntiles);
 
