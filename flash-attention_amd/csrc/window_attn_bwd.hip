@@ -19,7 +19,7 @@
 // its keys fill the registers) and forms S and dP for each half again.
 // Measured, bf16, B 4, 32 heads on 8 of 4096 positions, d 128, window 1024, 4 sinks: dQ 404 us, dK, dV 551, join 5.5; that is
 // 895 and 875 TFLOP/s of the three and four products (those of S and dP are formed twice; one kernel for all would have
-// to add dQ up with atomics, in no fixed order).  Matrix pipe busy 47 % and 50 % of the cycles, at the clock that the power
+// to add dQ up with atomics, in no fixed order).  Matrix pipe busy 50 % and 51 % of the cycles, at the clock that the power
 // limit leaves on random operands.
 // P and dS are rounded to the element type as operands; everything else is float32.  Rows and keys that
 // have no visible partner in the workgroup are fetched as zeros, so whatever stands there stays out; what some of its
