@@ -14,7 +14,7 @@
 // shares' unnormalised sums, in order.  With `weight_sum`, the logits are kept in the workspace (4 bytes per
 // head and key against 4 d read) and the second launch adds exp(logit - lse), summed over the group's heads in
 // order, to the running sum of each key.
-// Measured, 32 heads on 8, d 128: 8 sequences of up to 131072 keys (f16, 2.7 GB) 485 us = 5.65 TB/s, what a sum over a large
+// Measured, 32 heads on 8, d 128: 8 sequences of up to 131072 keys (f16, 2.7 GB) 476 us = 5.76 TB/s, what a sum over a large
 // tensor reaches; 64 of up to 4096 with weights (bf16, 615 MB) 157 us = 3.9 TB/s, of which the join and the weights take
 // 13; one sequence of 1024 keys 12.3 us: two launches, 9.4 us of dependent loads (table, keys, values) and 2.5 us of join.
 // Append: 64 tokens 4.2 us (a launch); 8 prompts of 4096 (268 MB) 55 us = 4.9 TB/s.
@@ -61,10 +61,21 @@ __device__ __forceinline__ f32x4 mma16_chunk(typename DFrag<T>::type a, typename
 // swizzle of a V row's 16-byte chunks: eight rows of the same two columns of chunks on different banks
 template <int RB> __device__ __forceinline__ int v_swz(int row) { return RB == 128 ? ((row >> 1) & 3) << 5 : (row & 7) << 5; }
 
+// The sequence that is `slot`-th in length, so that the launch does not end with long ones.
+__device__ __forceinline__ int longest_first(const DecodeShape& w, int slot, int lane) {
+    const int len = lane < w.B ? max(w.lens[lane], 0) : -1;
+    int before = 0;
+    for (int x = 0; x < w.B; ++x) {
+        const int other = __builtin_amdgcn_readlane(len, x);
+        before += (other > len) | ((other == len) & (x < lane));
+    }
+    return (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(before == slot && lane < w.B));
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(256, D * sizeof(T) <= 256 ? 3 : 1)
 paged_decode_kernel(const T* __restrict__ Qg, PagedCache c, T* __restrict__ Og, float* __restrict__ LSEg, DecodeShape w,
-                    int qtiles, int ns, float* __restrict__ part_o, float* __restrict__ part_ml,
+                    int qtiles, int ns, bool ranked, float* __restrict__ part_o, float* __restrict__ part_ml,
                     float* __restrict__ scores, int64_t score_row) {
     using frag = typename DFrag<T>::type;
     constexpr int RB = D * (int)sizeof(T), KS = RB / 64, DB = D / 16, EPC = 16 / (int)sizeof(T);
@@ -78,7 +89,7 @@ paged_decode_kernel(const T* __restrict__ Qg, PagedCache c, T* __restrict__ Og, 
     const int part = blockIdx.x % ns;
     int u = blockIdx.x / ns;
     const int qt = u % qtiles; u /= qtiles;
-    const int kvh = u % w.Hkv, b = u / w.Hkv, group = w.H / w.Hkv;
+    const int kvh = u % w.Hkv, b = ranked ? longest_first(w, u / w.Hkv, lane) : u / w.Hkv, group = w.H / w.Hkv;
     const int heads = min(16, group - 16 * qt);                       // query heads of this workgroup
     const int head0 = kvh * group + 16 * qt;
 
@@ -379,13 +390,16 @@ paged_append_kernel(const char* __restrict__ kn, const char* __restrict__ vn, ch
 // ---------------------------------------------------------------- host
 int pad_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-struct DecodePlan { int ns, D, qtiles; int64_t score_row, ml_floats, o_floats, score_floats; };
+struct DecodePlan { int ns, D, qtiles; bool ranked; int64_t score_row, ml_floats, o_floats, score_floats; };
 
 // Shares per head: enough workgroups that the chip is full several times over (the lengths are on the device, and
 // sequences differ), as long as every wave of a share has two tiles of the longest possible sequence; one share where
 // its waves have four tiles or fewer, which saves the second launch.  Measured (us, workgroups aimed at 1024 / 2048 /
 // 4096 / 8192): 8 sequences up to 131072 keys 499 / 505 / 485 / 503, 64 up to 4096 171 / 157 / 153 / 157; tiles per
 // wave 1 / 2 / 4 / 8: one sequence of 1024 keys 12.3 / 12.7 / 17.1 / 23.2; at most 300 keys, split / not: 12.7 / 10.3.
+// Sequences go longest first (batches of up to a wave's lanes) where a share of the longest possible one is long: measured, as they
+// come / longest first, tiles a share: 16 sequences of up to 32768 keys 235 / 220 (32), 64 of 8192 212 / 202 (32), 32 of 16384
+// 219 / 209 (32), 8 of 131072 484 / 476 (64); 64 of 4096 with weights 157 / 160 (16), 32 of 4096 52 / 59 (8: a tail of short ones).
 DecodePlan decode_plan(const DecodeShape& w, int64_t cap, bool weights) {
     DecodePlan p;
     p.D = pad_dim(w.d);
@@ -398,6 +412,7 @@ DecodePlan decode_plan(const DecodeShape& w, int64_t cap, bool weights) {
     if (ns > most) ns = most;
     if (ns > 128) ns = 128;
     p.ns = (int)(ns < 1 ? 1 : ns);
+    p.ranked = w.B > 1 && w.B <= 64 && tiles / p.ns >= 32;
     const int64_t bh = (int64_t)w.B * w.H;
     p.score_row = weights ? cdiv(cap, kKeys) * kKeys : 0;
     p.ml_floats = p.ns > 1 || weights ? cdiv(bh * p.ns * 2, 4) * 4 : 0;
@@ -418,7 +433,7 @@ int launch_decode(const void* q, const PagedCache& c, void* o, float* lse, float
     float* scores = weight_sum ? ws + p.o_floats + p.ml_floats : nullptr;
     auto go = [&](auto kern) {
         launch_kernel(kern, dim3((unsigned)nwg), dim3(256), 0, s, static_cast<const T*>(q), c, static_cast<T*>(o), lse, w,
-                      p.qtiles, p.ns, ws, ml, scores, p.score_row);
+                      p.qtiles, p.ns, p.ranked, ws, ml, scores, p.score_row);
     };
     if (p.D == 64) go(paged_decode_kernel<T, 64>);
     else if (p.D == 128) go(paged_decode_kernel<T, 128>);

@@ -121,6 +121,15 @@ def test_decode_long_and_split(mfa):
     _check_decode(mfa, [9000, 40], 4, 1, 32, 128, 2000, 4, F16, False)
 
 
+@pytest.mark.parametrize("B,weights", [(40, False), (64, True), (65, False)])
+def test_decode_many_sequences_of_unlike_lengths(mfa, B, weights):
+    """Batches large and long enough that the sequences go longest first, with equal lengths and empty ones among them; and one
+    sequence too many for that."""
+    lens = [(37 * b * b) % 300 for b in range(B)]
+    lens[7], lens[B - 1], lens[3], lens[4] = 4300, 0, 120, 120
+    _check_decode(mfa, lens, 32, 32, 16, 16, 0, 0, BF16, weights)
+
+
 def test_decode_table_wider_than_needed(mfa):
     _check_decode(mfa, [100, 20], 4, 2, 16, 64, 0, 0, BF16, True, width=400)
 
