@@ -451,6 +451,11 @@ window_bwd_dq_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
     }
     const int64_t orow = (int64_t)bh * w.Nq + row;
     const RowStat stat = row_stat<T>(of, Og + orow * w.d, LSEg + orow, live, w.d, h, st, rows, (int64_t)bh * nqp + qrow, wave == 0 && qrow < nqp);
+    // the rows between the last workgroup's 32 and nqp are nobody's else: dK, dV reads 64 at a time
+    if (wave == 0 && h == 0 && q0 + 32 >= w.Nq && qrow + 32 < nqp) {
+        st[(int64_t)bh * nqp + qrow + 32] = INFINITY;
+        st[rows + (int64_t)bh * nqp + qrow + 32] = 0.f;
+    }
     const float sl2 = w.scale * kLog2eW;
 
     f32x16 dq[R::DB];

@@ -448,3 +448,50 @@ def test_empty_sizes(mfa):
     assert out.shape == (1, 2, 0, 64)
     dq, dk, dv = mfa.window_attn_bwd(out, q, k, k, out, lse, 4, sinks=1)
     assert dq.numel() == 0 and not dk.any() and not dv.any()
+
+
+def _bwd_with_workspace(dout, q, k, v, out, lse, window, sinks, scale, lens, fill):
+    """window_attn_bwd through the C entry, its workspace holding nothing but float32 `fill` before the call."""
+    import ctypes
+
+    from my_flash_attn_cuda import _lib
+    B, H, nq, d = q.shape
+    G, nk = k.shape[1:3]
+    tag = {F32: _lib.MYFA_F32, F16: _lib.MYFA_F16, BF16: _lib.MYFA_BF16}[q.dtype]
+    nbytes = _lib.lib.myfa_window_attn_bwd_ws_bytes(B, H, G, nq, nk, d, window, sinks, tag)
+    ws = torch.full((nbytes // 4,), fill, device="cuda")
+    grads = [torch.empty_like(t) for t in (q, k, v)]
+    strides = [(ctypes.c_int64 * 3)(*t.stride()[:3]) for t in (q, k, v)]
+    _lib.check(_lib.lib.myfa_window_attn_bwd(
+        *(t.data_ptr() for t in (q, k, v, out, lse, dout, *grads)), None if lens is None else lens.data_ptr(),
+        B, H, G, nq, nk, d, *strides, window, sinks, scale, tag, ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream))
+    return dict(zip(("dq", "dk", "dv"), grads))
+
+
+@pytest.mark.parametrize("case", [
+    # few query blocks that meet many key blocks, the last rows of a head filling at most half of the 64 that dK, dV reads at a time
+    (1, 8, 8, 1044, 1044, 128, 300, 0, None, BF16),
+    (1, 8, 8, 1044, 1044, 128, 300, 4, None, F16),
+    (1, 8, 8, 20, 1200, 128, 150, 3, None, BF16),
+    (2, 8, 8, 70, 1100, 128, 2000, 0, [1100, 1050], BF16),
+    (1, 8, 8, 65, 3300, 64, 400, 2, None, F16),
+    (1, 64, 64, 20, 1100, 16, 200, 1, None, F32),
+    (1, 4, 4, 33, 4200, 192, 500, 1, None, BF16),
+    (1, 4, 2, 100, 100, 64, 30, 2, [90], BF16),              # few of both
+    (2, 96, 48, 161, 300, 64, 64, 4, [300, 170], BF16),      # many of both
+], ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+def test_gradients_do_not_depend_on_the_workspace(mfa, case):
+    B, H, G, nq, nk, d, window, sinks, lens, dtype = case
+    q, k, v, dout = _inputs(B, H, G, nq, nk, d, dtype, 11)
+    scale = d ** -0.5
+    want = ref.attention(q, k, v, _visible(B, nq, nk, window, sinks, lens), scale, dtype, dout)
+    q, k, v, dout = (t.cuda() for t in (q, k, v, dout))
+    L = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out, lse = mfa.window_attn_fwd(q, k, v, window, sinks=sinks, scale=scale, return_lse=True, seq_lens=L)
+    zeros = _bwd_with_workspace(dout, q, k, v, out, lse, window, sinks, scale, L, 0.0)
+    for name in zeros:
+        ref.check(name, zeros[name], want[name])
+    for fill in (float("nan"), float("inf"), -1e30):
+        again = _bwd_with_workspace(dout, q, k, v, out, lse, window, sinks, scale, L, fill)
+        for name in zeros:
+            assert torch.equal(again[name], zeros[name]), (name, fill)
