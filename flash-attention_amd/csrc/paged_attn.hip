@@ -275,13 +275,14 @@ paged_decode_kernel(const T* __restrict__ Qg, PagedCache c, T* __restrict__ Og, 
         if (ns > 1) {
             *reinterpret_cast<f32x4*>(part_o + (bh * ns + part) * D + col) = sum;
         } else {
-            const float inv = sn.len > 0 ? 1.f / total : 0.f;
+            const bool any = (sn.len > 0) | sn.past;             // (past: NaN, with a table of no pages too)
+            const float inv = any ? 1.f / total : 0.f;
             typedef T vec4 __attribute__((ext_vector_type(4)));
             vec4 y;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[r] = sn.len > 0 ? (T)(sum[r] * inv) : (T)0.f;
+            for (int r = 0; r < 4; ++r) y[r] = any ? (T)(sum[r] * inv) : (T)0.f;
             if (col < w.d) *reinterpret_cast<vec4*>(Og + bh * w.d + col) = y;
-            if (col == 0 && LSEg != nullptr) LSEg[bh] = sn.len > 0 ? (top + __builtin_amdgcn_logf(total)) * kLn2P : -INFINITY;
+            if (col == 0 && LSEg != nullptr) LSEg[bh] = any ? (top + __builtin_amdgcn_logf(total)) * kLn2P : -INFINITY;
         }
     }
 }

@@ -514,3 +514,14 @@ def test_empty_batch(mfa):
     sums, lens, kept = mfa.paged_kv_evict(k_pool, k_pool, torch.zeros(0, 2, 48, device="cuda"), table, L,
                                           torch.zeros(0, 2, device="cuda", dtype=torch.int32), 20)
     assert sums.shape == (0, 2, 32) and lens.shape == (0,) and kept.shape == (0, 2, 20)
+
+
+@pytest.mark.parametrize("weights", [False, True])
+def test_decode_with_no_pages_at_all(mfa, weights):
+    """A table of width 0 holds nothing: a length of 0 gives 0, any other lies beyond the capacity."""
+    k_pool = torch.zeros(4, 2, 16, 64, device="cuda", dtype=BF16)
+    q = torch.ones(3, 4, 64, device="cuda", dtype=BF16)
+    sums = torch.zeros(3, 2, 0, device="cuda") if weights else None
+    out, lse = mfa.paged_attn_decode(q, k_pool, k_pool, _i32([[], [], []]), _i32([0, 1, 40]), weight_sum=sums, return_lse=True)
+    assert not out[0].any() and (lse[0] == float("-inf")).all()
+    assert torch.isnan(out[1:]).all() and torch.isnan(lse[1:]).all()
