@@ -77,6 +77,8 @@ int paged_evict(const PagedCache& c, const EvictShape& e, hipStream_t s);
 namespace {
 
 constexpr int64_t kMaxCount = 1 << 28;     // tokens of a sequence, and batch, heads, ... each: products of two fit 64 bits
+// keys of a paged sequence: the kernels' 32-bit loops step up to 8192 keys past the last one
+constexpr int64_t kMaxCapacity = (1ll << 31) - (1 << 16);
 
 int elem_size(int dtype) { return dtype == MYFA_F32 ? 4 : 2; }
 bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; }
@@ -143,7 +145,7 @@ int paged_cache(const char* what, PagedCache& c, const void* k, const void* v, c
     for (int64_t x : {B, Hkv, num_pages, width, page})
         if (x > kMaxCount) return fail(MYFA_E_UNSUPPORTED, "%s: size %lld beyond 2^28", what, (long long)x);
     if (B * Hkv > kMaxCount) return fail(MYFA_E_UNSUPPORTED, "%s: %lld heads", what, (long long)(B * Hkv));
-    if (width * page >= 1ll << 31) return fail(MYFA_E_UNSUPPORTED, "%s: capacity of %lld keys a sequence", what, (long long)(width * page));
+    if (width * page > kMaxCapacity) return fail(MYFA_E_UNSUPPORTED, "%s: capacity of %lld keys a sequence", what, (long long)(width * page));
     if (int rc = check_elem(what, d, dtype)) return rc;
     if (int rc = check_strides(what, "the key cache", ks, 3, dtype)) return rc;
     if (int rc = check_strides(what, "the value cache", vs, 3, dtype)) return rc;
@@ -417,7 +419,7 @@ int decode_shape(const char* what, DecodeShape& w, int64_t B, int64_t H, int64_t
 int64_t myfa_paged_attn_decode_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t d, int64_t page, int64_t table_width,
                                         int64_t window, int64_t sinks, int with_weights) {
     DecodeShape w;
-    if (page < 1 || page > kMaxCount || table_width < 0 || table_width > kMaxCount || page * table_width >= 1ll << 31 || d > 256) return 0;
+    if (page < 1 || page > kMaxCount || table_width < 0 || table_width > kMaxCount || page * table_width > kMaxCapacity || d > 256) return 0;
     if (decode_shape("paged attention", w, B, H, Hkv, d, window, sinks, page * table_width) != MYFA_OK) return 0;
     if (B == 0 || d == 0) return 0;
     return paged_decode_ws_bytes(w, page * table_width, with_weights != 0);
@@ -457,7 +459,7 @@ int myfa_paged_evict(void* k_cache, void* v_cache, const float* weight_sum, cons
     const char* what = "paged eviction";
     PagedCache c;
     if (int rc = paged_cache(what, c, k_cache, v_cache, block_table, B, Hkv, d, num_pages, page, table_width, kc_strides, vc_strides, dtype)) return rc;
-    if (new_width < 0 || new_width > kMaxCount || new_width * page >= 1ll << 31) return fail(MYFA_E_UNSUPPORTED, "%s: new table of %lld pages", what, (long long)new_width);
+    if (new_width < 0 || new_width > kMaxCount || new_width * page > kMaxCapacity) return fail(MYFA_E_UNSUPPORTED, "%s: new table of %lld pages", what, (long long)new_width);
     if (budget < 1 || sinks < 0 || recent < 0 || sinks > budget || recent > budget - sinks)
         return fail(MYFA_E_INVALID, "%s: budget %lld must be at least 1 and hold sinks (%lld) and recent (%lld)", what, (long long)budget,
                     (long long)sinks, (long long)recent);

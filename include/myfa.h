@@ -321,7 +321,7 @@ int myfa_window_attn_bwd(const void* q, const void* k, const void* v, const void
  * A paged key/value cache: pools k_cache and v_cache of `num_pages` pages [num_pages, Hkv, page, d], each with
  * strides {page, head, slot} in elements (host array; the last dimension dense, all multiples of 16 bytes).  Key j
  * of sequence b stands in page block_table[b][j / page], slot j % page; block_table is int32 [B, table_width] on the
- * device.  Sequences hold at most capacity = table_width * page keys (< 2^31).  Entries behind a sequence's last
+ * device.  Sequences hold at most capacity = table_width * page keys (at most 2^31 - 2^16).  Entries behind a sequence's last
  * page are not read.  A page number outside [0, num_pages) is never turned into an address.
  * Element types as in myfa_window_attn_fwd.
  */

@@ -136,3 +136,25 @@ def test_reference_masks():
     """The definition the GPU tests are held to, on a case small enough to see."""
     got = ref.seen(3, 5, 2, 1, 4).int().tolist()      # positions 2, 3, 4; length 4
     assert got == [[1, 1, 1, 0, 0], [1, 0, 1, 1, 0], [0, 0, 0, 0, 0]]
+
+
+def test_capacities_that_32_bit_loops_cannot_walk_are_refused():
+    """A loop over keys steps past the last one before it ends: close to 2^31 it would wrap and not end.  (Null pointers: what the sizes
+    let through stops there, and nothing is launched.)"""
+    lib, bf16 = _lib.lib, _lib.MYFA_BF16
+    st = S3(2 * 16 * 64, 16 * 64, 64)
+    limit = (1 << 31) - (1 << 16)
+
+    def calls(page, width, new_width):
+        yield lib.myfa_paged_append(*[None] * 7, 1, 2, 1, 64, 8, page, width, st, st, st, st, bf16, None)
+        yield lib.myfa_paged_attn_decode(*[None] * 8, 1, 4, 2, 64, 8, page, width, st, st, st, 0, 0, 1.0, bf16, None, 0, None)
+        yield lib.myfa_paged_evict(*[None] * 9, 1, 2, 64, 8, page, width, new_width, st, st, 1, 0, 0, bf16, None)
+    for page, width in ((16, (1 << 27) - 1), (1 << 16, (1 << 15) - 1), (1, (1 << 28)), (1 << 28, 7), (16, limit // 16 + 1)):
+        for rc in calls(page, width, 1):
+            if page * width > limit:
+                _error(rc, 2, "capacity")
+            else:
+                _error(rc, 1, "null")
+        assert (lib.myfa_paged_attn_decode_ws_bytes(1, 4, 2, 64, page, width, 0, 0, 0) > 0) == (page * width <= limit)
+    _error(list(calls(16, 4, limit // 16 + 1))[2], 2, "new table")
+    _error(list(calls(16, 4, limit // 16))[2], 1, "null")
