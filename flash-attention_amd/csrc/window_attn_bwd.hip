@@ -1196,7 +1196,11 @@ template <typename T, int D> struct Large {
 struct BwdPlan { bool few_q, few_k; int bk, nqp, nkblk, nsb, ns; int64_t rows, stat_floats, part_floats; };
 
 // How many workgroups share a key block with sinks: enough that none has more than about a plain block's
-// queries, at most 32 (the parts are written and read once more).
+// queries, at most 32 (the parts are written and read once more).  Where many blocks hold sinks there is less to even out, and
+// the parts are bounded: they hold as many rows as there are keys, or come from at most 1024 workgroups (four a CU).  Measured, bf16,
+// d 128, window 256, without the bound / with: B 4, 32 heads on 8 of 16384 positions, 8192 sinks 27.5 ms and 8.6 GB of workspace / 21.1 ms
+// and 554 MB; B 1, 8 heads of 8192, 1024 sinks 268 us, 185 MB / 239 us, 135 MB; one head of 16384, 4000 sinks 210 us both.
+constexpr int64_t kSplitUnits = 1024;
 BwdPlan bwd_plan(const WindowShape& w, int elem_size) {
     BwdPlan p;
     p.few_q = few_queries(w);
@@ -1208,7 +1212,12 @@ BwdPlan bwd_plan(const WindowShape& w, int elem_size) {
     const bool uneven = w.sinks > 0 && w.window + p.bk < w.Nk;
     p.nsb = uneven ? (int)cdiv(w.sinks, p.bk) : 0;
     const int64_t each = cdiv(w.Nk, (int64_t)w.window + p.bk);
-    p.ns = p.nsb > 0 ? (int)(each < 32 ? each : 32) : 1;
+    int64_t most = 32;
+    if (p.nsb > 0) {
+        const int64_t rows = p.nkblk / p.nsb, units = kSplitUnits / ((int64_t)w.B * w.Hkv * p.nsb), bound = rows > units ? rows : units;
+        if (bound < most) most = bound > 1 ? bound : 1;
+    }
+    p.ns = p.nsb > 0 ? (int)(each < most ? each : most) : 1;
     p.stat_floats = 2 * p.rows;
     p.part_floats = p.ns > 1 ? (int64_t)w.B * w.Hkv * p.nsb * p.ns * 2 * p.bk * w.d : 0;
     return p;

@@ -306,7 +306,9 @@ int myfa_window_attn_fwd(const void* q, const void* k, const void* v, void* o, f
  * that see nothing are 0.  A row of q, k, v or dout that is not finite makes the gradients of the rows and keys it is
  * seen with so, and no others.  `workspace`: myfa_window_attn_bwd_ws_bytes(...) bytes, 16-byte aligned, whose contents
  * before and after mean nothing; it must stay untouched until the call's work on `stream` has finished, and
- * calls that may overlap need one each.  No atomics: the result depends on the inputs alone.
+ * calls that may overlap need one each.  It holds two floats a query row (of every head, rows rounded up to 64) and, where the
+ * sinks' keys are split, float32 parts of dk and dv of at most the larger of (Nk + 127) rows a head and 1024 x 128 rows in all.
+ * No atomics: the result depends on the inputs alone.
  */
 int64_t myfa_window_attn_bwd_ws_bytes(int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nk, int64_t d,
                                       int64_t window, int64_t sinks, int dtype);

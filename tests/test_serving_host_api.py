@@ -158,3 +158,23 @@ def test_capacities_that_32_bit_loops_cannot_walk_are_refused():
         assert (lib.myfa_paged_attn_decode_ws_bytes(1, 4, 2, 64, page, width, 0, 0, 0) > 0) == (page * width <= limit)
     _error(list(calls(16, 4, limit // 16 + 1))[2], 2, "new table")
     _error(list(calls(16, 4, limit // 16))[2], 1, "null")
+
+
+def test_workspace_of_the_window_backward_is_bounded():
+    """However many keys are sinks: statistics of every query row, and parts as include/myfa.h bounds them."""
+    rng = random.Random(1)
+    shapes = [(4, 8, 8, 16384, 128, 256, 8192), (4, 8, 8, 16384, 128, 16, 16384), (1, 1, 1, 16384, 256, 100, 4000), (64, 8, 8, 16384, 128, 256, 4),
+              (4, 32, 8, 4096, 128, 1024, 4), (1, 2, 1, 640, 64, 100, 130)]
+    for _ in range(2000):
+        nk, G = int(2 ** rng.uniform(0, 18)), rng.choice([1, 2, 3, 8, 32])
+        shapes.append((int(2 ** rng.uniform(0, 7)), G * rng.choice([1, 2, 8]), G, nk, rng.choice([8, 64, 80, 128]), int(2 ** rng.uniform(0, 18)),
+                       rng.choice([0, 1, 4, 100, nk // 2, nk, 1 << 40])))
+    split = 0
+    for B, H, G, nk, d, window, sinks in shapes:
+        for dtype in (_lib.MYFA_BF16, _lib.MYFA_F32) if d <= 128 else (_lib.MYFA_BF16,):
+            nq = rng.randrange(1, nk + 1)
+            got = _lib.lib.myfa_window_attn_bwd_ws_bytes(B, H, G, nq, nk, d, window, sinks, dtype)
+            stats = 8 * B * H * (-(-nq // 64) * 64)
+            assert stats <= got <= stats + 2 * 4 * d * max(B * G * (nk + 127), 1024 * 128), (B, H, G, nq, nk, d, window, sinks)
+            split += got > stats
+    assert split > 200

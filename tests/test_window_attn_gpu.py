@@ -495,3 +495,10 @@ def test_gradients_do_not_depend_on_the_workspace(mfa, case):
         again = _bwd_with_workspace(dout, q, k, v, out, lse, window, sinks, scale, L, fill)
         for name in zeros:
             assert torch.equal(again[name], zeros[name]), (name, fill)
+
+
+@pytest.mark.parametrize("case", [(4, 16, 16, 300, 300, 64, 20, 150, None), (2, 32, 16, 500, 500, 64, 20, 400, [500, 310]), (16, 32, 32, 200, 200, 16, 20, 190, None),
+                                  (1, 2, 1, 900, 900, 128, 20, 300, None)], ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+def test_many_sinks(mfa, case):
+    """Several key blocks of sinks, split as far as the bound on the workspace lets them, or not at all."""
+    _compare(mfa, *case, BF16)
