@@ -113,6 +113,25 @@ def _load():
 lib = _load()
 
 
+class _NoHost:
+    """In the place of the host extension module where that does not load: it is tied to one Python and one torch, the
+    library above is not, so dense attention and softmax go on and the operators that need the module say why they do not."""
+
+    def __init__(self, why):
+        self._why = why
+
+    def __getattr__(self, name):
+        if name.startswith("__"):
+            raise AttributeError(name)
+        raise RuntimeError(f"{name}: the host extension module _host.so does not load here ({self._why}); rebuild it with flash-attention_amd/build.py")
+
+
+try:
+    from . import _host as host
+except ImportError as e:
+    host = _NoHost(str(e))
+
+
 def check(status):
     """Turns a nonzero C status into RuntimeError (what the reference's TORCH_CHECK
     failures surface as in Python)."""

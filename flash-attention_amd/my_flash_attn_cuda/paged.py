@@ -7,7 +7,7 @@ holds at most width * page keys, its capacity.  Lengths and tables stay on the d
 and every call can be captured into a graph.  Page numbers outside the pool never become addresses.
 The reference has no cache (csrc/api.cpp:168-192 takes whole matrices).
 """
-from . import _host
+from ._lib import host as _host
 
 
 def paged_kv_append(k, v, k_cache, v_cache, block_table, seq_lens, counts=None):

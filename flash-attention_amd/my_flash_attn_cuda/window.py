@@ -3,7 +3,7 @@
 The reference's attention sees every key (csrc/api.cpp:168-192); this is the form that decoders with long
 contexts use, beside flash_attn_fwd / flash_attn_bwd / flash_attn_func and in their manner.
 """
-from . import _host
+from ._lib import host as _host
 
 
 def window_attn_fwd(q, k, v, window, sinks=0, scale=1.0, return_lse=False, seq_lens=None):

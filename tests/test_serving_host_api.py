@@ -178,3 +178,36 @@ def test_workspace_of_the_window_backward_is_bounded():
             assert stats <= got <= stats + 2 * 4 * d * max(B * G * (nk + 127), 1024 * 128), (B, H, G, nq, nk, d, window, sinks)
             split += got > stats
     assert split > 200
+
+
+@pytest.mark.parametrize("host", ["none", "other"])
+def test_the_package_without_its_host_module(tmp_path, host):
+    """Where the extension module is absent, or is of another torch, dense attention and softmax are there as before it existed, and the
+    operators that need it say so."""
+    import os
+    import subprocess
+    import sys
+    src, pkg = os.path.dirname(_lib.__file__), tmp_path / "my_flash_attn_cuda"
+    pkg.mkdir()
+    for name in os.listdir(src):
+        if name.endswith(".py") or name == "libmyfa_gfx950.so":
+            os.symlink(os.path.join(src, name), pkg / name)
+    if host == "other":
+        (pkg / "_host.so").write_bytes(b"not for this Python")
+    code = """
+import torch, my_flash_attn_cuda as m
+assert m._lib.__file__.startswith(%r)
+x, i = torch.zeros(1, 2, 8, 64), torch.zeros(1, 2, dtype=torch.int32)
+def message(call):
+    try:
+        call()
+    except RuntimeError as e:
+        return str(e)
+for call in (lambda: m.flash_attn_fwd(x, x, x), lambda: m.softmax(x, -1), lambda: m.my_softmax(x[0, 0], 5)):
+    assert "must be a CUDA tensor" in message(call), message(call)
+for call in (lambda: m.window_attn_fwd(x, x, x, 4), lambda: m.window_attn_func(x, x, x, 4), lambda: m.window_attn_bwd(x, x, x, x, x, x, 4),
+             lambda: m.paged_kv_append(x, x, x, x, i, i[0]), lambda: m.paged_attn_decode(x[0], x, x, i, i[0]), lambda: m.paged_kv_evict(x, x, x, i, i[0], i, 4)):
+    assert "_host.so does not load" in message(call), message(call)
+""" % str(tmp_path)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=tmp_path, env={**os.environ, "PYTHONPATH": str(tmp_path)})
+    assert r.returncode == 0, r.stderr
