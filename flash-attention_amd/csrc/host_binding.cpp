@@ -84,6 +84,11 @@ struct Strides {
     }
 };
 
+// A tensor that a call has written in place, for the graphs that saved it.  (Tensors of inference mode have no version.)
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 const int32_t* ints(const OptTensor& t) { return t.has_value() ? t->const_data_ptr<int32_t>() : nullptr; }
 
 // ---------------------------------------------------------------- window attention
@@ -231,6 +236,8 @@ void paged_kv_append(const Tensor& k, const Tensor& v, const Tensor& kc, const T
     const c10::DeviceGuard guard(kc.device());
     check(myfa_paged_append(k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(), table.const_data_ptr<int32_t>(), lens.const_data_ptr<int32_t>(), ints(counts),
                             c.B, c.heads, k.size(2), c.d, c.pages, c.page, c.width, ks.s, vs.s, c.ks.s, c.vs.s, tag(kc), current_stream(kc)));
+    written(kc);
+    written(vc);
 }
 
 py::object paged_attn_decode(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& lens, double scale, py::handle window_,
@@ -255,6 +262,7 @@ py::object paged_attn_decode(const Tensor& q, const Tensor& kc, const Tensor& vc
                                  want_lse ? lse.data_ptr<float>() : nullptr, sums.has_value() ? sums->data_ptr<float>() : nullptr, c.B, H, c.heads, c.d,
                                  c.pages, c.page, c.width, qs.s, c.ks.s, c.vs.s, window, sinks, (float)scale, tag(q), bytes > 0 ? ws.data_ptr() : nullptr, bytes,
                                  current_stream(kc)));
+    if (sums.has_value()) written(*sums);
     if (!want_lse) return py::cast(out);
     return py::make_tuple(out, lse);
 }
@@ -275,6 +283,8 @@ py::tuple paged_kv_evict(const Tensor& kc, const Tensor& vc, const Tensor& sums,
     check(myfa_paged_evict(kc.data_ptr(), vc.data_ptr(), sums.const_data_ptr<float>(), table.const_data_ptr<int32_t>(), lens.const_data_ptr<int32_t>(),
                            new_table.const_data_ptr<int32_t>(), new_sums.data_ptr<float>(), new_lens.data_ptr<int32_t>(), kept.data_ptr<int32_t>(), c.B, c.heads, c.d,
                            c.pages, c.page, c.width, new_table.size(1), c.ks.s, c.vs.s, budget, sinks, recent, tag(kc), current_stream(kc)));
+    written(kc);
+    written(vc);
     return py::make_tuple(new_sums, new_lens, kept);
 }
 

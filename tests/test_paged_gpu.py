@@ -525,3 +525,36 @@ def test_decode_with_no_pages_at_all(mfa, weights):
     out, lse = mfa.paged_attn_decode(q, k_pool, k_pool, _i32([[], [], []]), _i32([0, 1, 40]), weight_sum=sums, return_lse=True)
     assert not out[0].any() and (lse[0] == float("-inf")).all()
     assert torch.isnan(out[1:]).all() and torch.isnan(lse[1:]).all()
+
+
+def test_writes_in_place_are_seen_by_autograd(mfa):
+    """What a call writes in place gets a new version, so that a graph that saved it is not run over other values."""
+    c = Cache([100, 40], 2, 16, 64, BF16, 14, spare=8, width=10)
+    for b in range(2):
+        c.table[b, -(-c.lens[b] // 16)] = c.free.pop()
+    new_table = torch.tensor([[c.free.pop(), c.free.pop()] for _ in range(2)], dtype=torch.int32, device="cuda")
+    k_pool, v_pool, table, L = c.gpu()
+    new = torch.ones(2, 2, 1, 64, device="cuda", dtype=BF16)
+    sums = torch.zeros(2, 2, 160, device="cuda")
+    calls = {
+        "append": (lambda: mfa.paged_kv_append(new, new, k_pool, v_pool, table, L), (k_pool, v_pool)),
+        "decode": (lambda: mfa.paged_attn_decode(new[:, :, 0], k_pool, v_pool, table, L, weight_sum=sums), (sums,)),
+        "evict": (lambda: mfa.paged_kv_evict(k_pool, v_pool, sums, table, L, new_table, 32), (k_pool, v_pool)),
+    }
+    for name, (call, written) in calls.items():
+        everything = (k_pool, v_pool, sums, table, L, new_table, new)
+        before = [t._version for t in everything]
+        call()
+        for t, n in zip(everything, before):
+            assert (t._version > n) == any(t is x for x in written), name
+    w = torch.randn(k_pool.shape, device="cuda", dtype=BF16, requires_grad=True)
+    saved = (w * v_pool).sum()
+    mfa.paged_kv_append(new, new, k_pool, v_pool, table, L)
+    with pytest.raises(RuntimeError, match="inplace"):
+        saved.backward()
+    # tensors of inference mode have no version
+    with torch.inference_mode():
+        pools = [t.clone() for t in (k_pool, v_pool)]
+        mfa.paged_kv_append(new, new, *pools, table, L)
+    mfa.paged_kv_append(new, new, *pools, table, L)
+    assert torch.equal(pools[0].nan_to_num(9.0), k_pool.nan_to_num(9.0))
