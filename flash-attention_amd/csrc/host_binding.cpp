@@ -12,8 +12,10 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <optional>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "myfa.h"
@@ -84,6 +86,22 @@ struct Strides {
     }
 };
 
+// A tensor that a call is going to write in place: no history to keep, and no element in the place of another (two workgroups
+// would write there, in no order).  Sorted by stride, every dimension has to step over all that the smaller ones span, as
+// slices and transposes of dense tensors do.
+void check_target(const Tensor& t, const char* name) {
+    TORCH_CHECK(!(t.requires_grad() && at::GradMode::is_enabled()), name, " requires grad, and the call writes it in place without a history");
+    if (t.numel() == 0) return;
+    std::vector<std::pair<int64_t, int64_t>> dims;
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
+    std::sort(dims.begin(), dims.end());
+    int64_t span = 1;
+    for (const auto& [stride, size] : dims) {
+        TORCH_CHECK(stride >= span, name, " is written in place, but elements of it share memory (sizes ", t.sizes(), ", strides ", t.strides(), ")");
+        span += (size - 1) * stride;
+    }
+}
 // A tensor that a call has written in place, for the graphs that saved it.  (Tensors of inference mode have no version.)
 void written(const Tensor& t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -232,6 +250,7 @@ void paged_kv_append(const Tensor& k, const Tensor& v, const Tensor& kc, const T
     TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes() && k.size(0) == c.B && k.size(1) == c.heads && k.size(3) == c.d, "Wrong sizes!");
     TORCH_CHECK(k.scalar_type() == kc.scalar_type() && v.scalar_type() == kc.scalar_type(), "Scalar type mismatch!");
     if (counts.has_value()) check_ints(*counts, {c.B}, kc, "counts");
+    check_target(kc, "k_cache"); check_target(vc, "v_cache");
     const Strides ks(k, "k"), vs(v, "v");
     const c10::DeviceGuard guard(kc.device());
     check(myfa_paged_append(k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(), table.const_data_ptr<int32_t>(), lens.const_data_ptr<int32_t>(), ints(counts),
@@ -250,7 +269,10 @@ py::object paged_attn_decode(const Tensor& q, const Tensor& kc, const Tensor& vc
     const int64_t H = q.size(1), window = whole(window_, "window"), sinks = whole(sinks_, "sinks");
     TORCH_CHECK(H >= 1 && H % c.heads == 0, H, " query heads are not a multiple of ", c.heads, " key/value heads");
     TORCH_CHECK(window >= 0 && sinks >= 0, "window and sinks must be integers of at least 0, got ", window, " and ", sinks);
-    if (sums.has_value()) check_sums(*sums, {c.B, c.heads, c.width * c.page}, kc);
+    if (sums.has_value()) {
+        check_sums(*sums, {c.B, c.heads, c.width * c.page}, kc);
+        check_target(*sums, "weight_sum");
+    }
     const Strides qs(q, "q");
     const c10::DeviceGuard guard(kc.device());
     const auto opt = q.options().memory_format(at::MemoryFormat::Contiguous);
@@ -271,6 +293,7 @@ py::tuple paged_kv_evict(const Tensor& kc, const Tensor& vc, const Tensor& sums,
                          py::handle sinks_, py::handle recent_) {
     const Cache c = check_cache(kc, vc, table, lens);
     check_sums(sums, {c.B, c.heads, c.width * c.page}, kc);
+    check_target(kc, "k_cache"); check_target(vc, "v_cache");
     TORCH_CHECK(new_table.dim() == 2, "new_block_table must be an int32 (B, width) tensor");
     check_ints(new_table, {c.B, new_table.size(1)}, kc, "new_block_table");
     const int64_t budget = whole(budget_, "budget"), sinks = whole(sinks_, "sinks"), recent = whole(recent_, "recent"), capacity = new_table.size(1) * c.page;

@@ -5,6 +5,8 @@ every key/value head.  block_table, int32 (B, width), gives every sequence its p
 page block_table[b, j // page], slot j % page; entries behind a sequence's last page are not read.  A sequence
 holds at most width * page keys, its capacity.  Lengths and tables stay on the device: no call waits for the GPU,
 and every call can be captured into a graph.  Page numbers outside the pool never become addresses.
+What a call writes in place (the pools, weight_sum) has every element in memory of its own, and no history for autograd
+to keep: expanded views, and in grad mode tensors that require grad, are refused there.
 The reference has no cache (csrc/api.cpp:168-192 takes whole matrices).
 """
 from ._lib import host as _host

@@ -324,7 +324,8 @@ int myfa_window_attn_bwd(const void* q, const void* k, const void* v, const void
  * strides {page, head, slot} in elements (host array; the last dimension dense, all multiples of 16 bytes).  Key j
  * of sequence b stands in page block_table[b][j / page], slot j % page; block_table is int32 [B, table_width] on the
  * device.  Sequences hold at most capacity = table_width * page keys (at most 2^31 - 2^16).  Entries behind a sequence's last
- * page are not read.  A page number outside [0, num_pages) is never turned into an address.
+ * page are not read.  A page number outside [0, num_pages) is never turned into an address.  Where a call writes
+ * the cache, no two of its elements may share memory.
  * Element types as in myfa_window_attn_fwd.
  */
 

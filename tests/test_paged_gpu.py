@@ -558,3 +558,35 @@ def test_writes_in_place_are_seen_by_autograd(mfa):
         mfa.paged_kv_append(new, new, *pools, table, L)
     mfa.paged_kv_append(new, new, *pools, table, L)
     assert torch.equal(pools[0].nan_to_num(9.0), k_pool.nan_to_num(9.0))
+
+
+def test_writes_in_place_are_refused_where_they_cannot_be_made(mfa):
+    """A cache whose places share memory, and a tensor whose history autograd would have to keep."""
+    c = Cache([20, 20], 2, 16, 64, BF16, 15, spare=4)
+    k_pool, v_pool, table, L = c.gpu()
+    new = torch.ones(2, 2, 1, 64, device="cuda", dtype=BF16)
+    nt = torch.tensor([[c.free.pop()], [c.free.pop()]], dtype=torch.int32, device="cuda")
+    sums, q = torch.zeros(2, 2, 32, device="cuda"), torch.ones(2, 4, 64, device="cuda", dtype=BF16)
+    shared = [k_pool[:, :1].expand(-1, 2, -1, -1),                                                 # one head for all
+              k_pool[:1].expand(c.pages, -1, -1, -1),
+              torch.zeros(c.pages * 4096, device="cuda", dtype=BF16).as_strided(k_pool.shape, (2048, 1024, 32, 1))]     # rows half over each other
+    for x in shared:
+        for pools in ((x, v_pool), (v_pool, x)):
+            with pytest.raises(RuntimeError, match="share memory"):
+                mfa.paged_kv_append(new, new, *pools, table, L)
+            with pytest.raises(RuntimeError, match="share memory"):
+                mfa.paged_kv_evict(*pools, sums, table, L, nt, 16)
+        mfa.paged_attn_decode(q, x, x, table, L, weight_sum=sums)                                  # reads alone
+    grad = v_pool.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="requires grad"):
+        mfa.paged_kv_append(new, new, k_pool, grad, table, L)
+    with pytest.raises(RuntimeError, match="requires grad"):
+        mfa.paged_kv_evict(grad, k_pool, sums, table, L, nt, 16)
+    with pytest.raises(RuntimeError, match="requires grad"):
+        mfa.paged_attn_decode(q, k_pool, v_pool, table, L, weight_sum=sums.clone().requires_grad_())
+    with torch.no_grad():
+        mfa.paged_kv_append(new, new, k_pool, grad, table, L)
+    # (pages, page, heads, d) pools, interleaved ones and slices hold every place once
+    both = torch.zeros(c.pages, 16, 2, 2, 72, device="cuda", dtype=BF16)[..., :64]
+    mfa.paged_kv_append(new, new, both[:, :, 0].transpose(1, 2), both[:, :, 1].transpose(1, 2), table, L)
+    assert both.sum() == 2 * 2 * 2 * 64
