@@ -154,6 +154,7 @@ window_bwd_dq_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T
         }
     }
 
+    // (hidden dS are set to 0 behind the product with dP: hidden keys reach dQ, hidden values do not)
     const uint32_t redo = not_finite_rows(dq, live && finite(lse2) && finite(ndelta));
     if (qrow < w.Nq) {
         T* row = dQg + ((int64_t)bh * w.Nq + qrow) * w.d;
@@ -170,7 +171,7 @@ window_bwd_dq_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const T
             }
     }
     if (redo != 0) {                                        // (window_attn_exact.h)
-        const uint32_t cols = hidden_for_dq<T, D>(kt, w, q0 + 32 * wave + kt.shift, Kh, Vh, lane);
+        const uint32_t cols = hidden_keys<T, D>(kt, w, q0 + 32 * wave + kt.shift, Kh, w.ks[2], lane);
         stored();
         for (uint32_t left = any_lane(cols != 0) ? redo : 0; left != 0; left &= left - 1) {
             const int x = __builtin_ctz(left), i = q0 + 32 * wave + x;
@@ -368,6 +369,7 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
     }
     masked_tiles(min(max(f0, f1), ntiles), ntiles);
 
+    // (hidden dS are set to 0 behind the product with dP: hidden keys reach dQ, hidden values do not)
     const uint32_t redo = not_finite_rows(dq, live && finite(lse2) && finite(ndelta));
     if (qrow < w.Nq) {
         T* row = dQg + ((int64_t)bh * w.Nq + qrow) * w.d;
@@ -383,7 +385,7 @@ window_bwd_dq16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
             }
     }
     if (redo != 0) {                                        // (window_attn_exact.h)
-        const uint32_t cols = hidden_for_dq<T, D>(kt, w, q0 + 32 * wave + kt.shift, Kh, Vh, lane);
+        const uint32_t cols = hidden_keys<T, D>(kt, w, q0 + 32 * wave + kt.shift, Kh, w.ks[2], lane);
         stored();
         for (uint32_t left = any_lane(cols != 0) ? redo : 0; left != 0; left &= left - 1) {
             const int x = __builtin_ctz(left), i = q0 + 32 * wave + x;
@@ -485,7 +487,7 @@ window_bwd_dq_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
     }
 
     put_sums(reinterpret_cast<float*>(own), dq, r, h);
-    {
+    {                                                       // (hidden values do not reach dQ, as above)
         const uint32_t bad = not_finite_rows(dq, live && finite(stat.lse2) && finite(stat.ndelta));
         if (lane == 0) redo_of[wave] = bad;
     }
@@ -506,7 +508,7 @@ window_bwd_dq_few_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
         if (col < w.d) *reinterpret_cast<vec4*>(dQg + ((int64_t)bh * w.Nq + q0 + rw) * w.d + col) = y;
     }
     if (redo != 0) {                                        // (window_attn_exact.h)
-        const uint32_t cols = hidden_for_dq<T, D>(kt, w, q0 + kt.shift, Kh, Vh, lane);
+        const uint32_t cols = hidden_keys<T, D>(kt, w, q0 + kt.shift, Kh, w.ks[2], lane);
         stored();
         __syncthreads();
         int turn = 0;

@@ -163,13 +163,6 @@ __device__ __forceinline__ void exact_dq_row(const T* q, const T* dout, const T*
     dq.store(out, w.scale, cols, 0, w.d, lane);
 }
 
-// Columns of dQ that hidden keys reach: a value that is not finite makes the hidden dS NaN, and with it every column.
-template <typename T, int D, int BN>
-__device__ __forceinline__ uint32_t hidden_for_dq(const KeyTiles<BN>& kt, const WindowShape& w, int p0, const T* Kh, const T* Vh, int lane) {
-    if (any_lane(hidden_keys<T, D>(kt, w, p0, Vh, w.vs[2], lane) != 0)) return LaneRow<T, D>::all(w.d, lane);
-    return hidden_keys<T, D>(kt, w, p0, Kh, w.ks[2], lane);
-}
-
 // dK and dV of a key, a few queries at a time: rows q + x qs, dout + x d, statistics lse2[x], ndelta[x] for x < n
 template <typename T, int D> struct ExactKey {
     using L = LaneRow<T, D>;

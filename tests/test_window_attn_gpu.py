@@ -502,3 +502,22 @@ def test_gradients_do_not_depend_on_the_workspace(mfa, case):
 def test_many_sinks(mfa, case):
     """Several key blocks of sinks, split as far as the bound on the workspace lets them, or not at all."""
     _compare(mfa, *case, BF16)
+
+
+@pytest.mark.parametrize("shape", [(1, 4, 2, 260, 260, 64, 20, 0, BF16), (1, 2, 1, 200, 200, 128, 20, 2, F32), (1, 2, 1, 180, 180, 192, 20, 2, F16),     # few rows
+                                   (1, 100, 100, 260, 260, 128, 20, 3, F16), (1, 100, 100, 200, 200, 160, 20, 2, BF16)],
+                         ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+def test_a_hidden_value_does_not_change_a_bit_of_dq(mfa, shape):
+    """Where a hidden key's column is infinite already, and is formed again, an infinite value beside it changes nothing: hidden
+    weights are set to 0 behind the product that the value reaches.  (The forward forms such rows again, with other roundings: both
+    calls go by one out and lse.)"""
+    B, H, G, nq, nk, d, window, sinks, dtype = shape
+    q, k, v, dout = (t.cuda() for t in _inputs(B, H, G, nq, nk, d, dtype, 12))
+    at = 141
+    k[:, :, at, 5] = float("inf")
+    hidden = ~_visible(B, nq, nk, window, sinks, None)[0][:, at].cuda()
+    out, lse = mfa.window_attn_fwd(q, k, v, window, sinks=sinks, scale=0.125, return_lse=True)
+    first = mfa.window_attn_bwd(dout, q, k, v, out, lse, window, sinks=sinks, scale=0.125)[0][:, :, hidden]
+    v[:, :, at] = float("inf")
+    second = mfa.window_attn_bwd(dout, q, k, v, out, lse, window, sinks=sinks, scale=0.125)[0][:, :, hidden]
+    assert torch.isfinite(first).all() and torch.equal(first, second)
