@@ -168,6 +168,8 @@ window_attn_fwd_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, const
 //   maximum looked for, the running one moved, O and l rescaled and the weights formed again from the logits.
 //   Weights up to 2^8 are rounded with the same relative error, and neither the search for the maximum nor the
 //   rescale of O, 64 multiplications a lane, is in most tiles.
+//   Rows that see nothing (behind the length) have no vote, and waves of nothing but such rows no products: 16 heads of batches of 16,
+//   lengths 185 to 1100 of 1100, 110 us against 119 with them; lengths of whole blocks take the same time.
 //   The tiles that every row of the workgroup sees whole run in a loop without masks, bounds or tile arithmetic.
 // Measured (bf16, d 128): 16 heads of 16384 positions, window 4096: 452 us, 1065 TFLOP/s of what is seen, where a
 // library product of 8192^3 reaches 1194; B 4, 32 heads of 4096 positions, window 1024: 290 us, 832 (a tenth of the work
@@ -246,7 +248,8 @@ window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
                                    s[i / KS] = mma_chunk<T>(a, qf[i % KS], s[i / KS]);
                                }, [](auto) {});
     };
-    auto softmax = [&](f32x16 (&s)[2]) __attribute__((always_inline)) {
+    // votes: the lane's row sees something (rows that never do have no maximum to come)
+    auto softmax = [&](f32x16 (&s)[2], bool votes) __attribute__((always_inline)) {
         float sum[2];
         auto weights = [&](float ref) __attribute__((always_inline)) {
 #pragma unroll
@@ -260,7 +263,7 @@ window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
         };
         weights(m == -INFINITY ? 0.f : m);
         // (negated: a NaN or an infinite sum goes back too)
-        if (__builtin_amdgcn_ballot_w64(!(sum[0] + sum[1] <= 256.f) || m == -INFINITY) != 0) {
+        if (__builtin_amdgcn_ballot_w64(votes && (!(sum[0] + sum[1] <= 256.f) || m == -INFINITY)) != 0) {
             float a = vmax3(s[0][0], s[0][1], s[0][2]), c = vmax3(s[1][0], s[1][1], s[1][2]);
 #pragma unroll
             for (int i = 3; i < 15; i += 2) { a = vmax3(a, s[0][i], s[0][i + 1]); c = vmax3(c, s[1][i], s[1][i + 1]); }
@@ -295,14 +298,14 @@ window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
     auto masked_tiles = [&](int t0, int t1) __attribute__((always_inline)) {
         for (int t = t0; t < t1; ++t) {
             const int k0 = kt.first_key(t);
-            // something of this tile is seen by the wave's rows
-            const bool some = !(k0 > wave_hi || (k0 + BN <= wave_lo - w.window + 1 && k0 >= w.sinks));
+            // something of this tile is seen by the wave's rows (and some of them see anything)
+            const bool some = wave_lo < kt.pz && !(k0 > wave_hi || (k0 + BN <= wave_lo - w.window + 1 && k0 >= w.sinks));
             if (some) {
                 f32x16 s[2];
                 logits(lds + (t & 1) * TILE_B, s);
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) sees.hide(s[kb], kt, t, k0, k0 + 32 * kb + 4 * h, w.sinks, -INFINITY);
-                softmax(s);
+                softmax(s, live);
             }
             tile_ready();
             auto ahead = [&](auto ic) __attribute__((always_inline)) { if constexpr (decltype(ic)::value == 0) { fetch_v(t + 1); fetch_k(t + 2); } };
@@ -322,7 +325,7 @@ window_attn_fwd16_kernel(const T* __restrict__ Qg, const T* __restrict__ Kg, con
             for (int t = t0; t < t1; ++t) {
                 f32x16 s[2];
                 logits(lds + buf * TILE_B, s);
-                softmax(s);
+                softmax(s, true);
                 tile_ready();
                 add_pv(lds + (2 + buf) * TILE_B, [&](auto ic) __attribute__((always_inline)) {
                     constexpr int i = decltype(ic)::value, LPT = TileFetch<T, D, BN, 256>::LPT;

@@ -521,3 +521,17 @@ def test_a_hidden_value_does_not_change_a_bit_of_dq(mfa, shape):
     v[:, :, at] = float("inf")
     second = mfa.window_attn_bwd(dout, q, k, v, out, lse, window, sinks=sinks, scale=0.125)[0][:, :, hidden]
     assert torch.isfinite(first).all() and torch.equal(first, second)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_behind_the_length_do_not_change_the_others(mfa, d, dtype):
+    """The same bits whether the rows behind a row exist or not: with logits this small the running maximum stays where the first tile
+    leaves it (a lane's sum of 32 weights is below 2^8 everywhere), and rows that see nothing must not move it."""
+    q, k, v, _ = (t.cuda() for t in _inputs(1, 32, 32, 1024, 1024, d, dtype, 13))
+    out, lse = mfa.window_attn_fwd(q, k, v, 1024, scale=0.002, return_lse=True)
+    for n in (1000, 900, 897):
+        L = torch.tensor([n], dtype=torch.int32, device="cuda")
+        cut, cut_lse = mfa.window_attn_fwd(q, k, v, 1024, scale=0.002, return_lse=True, seq_lens=L)
+        assert torch.equal(cut[:, :, :n], out[:, :, :n]) and torch.equal(cut_lse[:, :, :n], lse[:, :, :n]), n
+        assert not cut[:, :, n:].any()
