@@ -343,6 +343,7 @@ int myfa_window_attn_fwd(const void* q, const void* k, const void* v, void* o, f
     WindowShape w;
     if (int rc = window_shape(what, w, seq_lens, B, H, Hkv, Nq, Nk, d, window, sinks, scale)) return rc;
     if (int rc = check_elem(what, d, dtype)) return rc;
+    if (d == 0 && lse) return fail(MYFA_E_UNSUPPORTED, "%s: head dim 0 has an output of no elements, but a log-sum-exp, which is not formed", what);
     if (B == 0 || Nq == 0 || d == 0) return MYFA_OK;
     if (!q || !k || !v || !o) return fail(MYFA_E_INVALID, "%s: null pointer", what);
     if (misaligned(q) || misaligned(k) || misaligned(v) || misaligned(o)) return fail(MYFA_E_INVALID, "%s: tensors must be 16-byte aligned", what);
@@ -437,6 +438,7 @@ int myfa_paged_attn_decode(const void* q, const void* k_cache, const void* v_cac
     DecodeShape w;
     if (int rc = decode_shape(what, w, B, H, Hkv, d, window, sinks, page * table_width)) return rc;
     if (!(scale > 0.f) || scale > 3e38f) return fail(MYFA_E_INVALID, "%s: scale must be positive and finite", what);
+    if (d == 0 && (lse || weight_sum)) return fail(MYFA_E_UNSUPPORTED, "%s: head dim 0 has an output of no elements, but a log-sum-exp and weights, which are not formed", what);
     if (B == 0 || d == 0) return MYFA_OK;
     if (!q || !o || !seq_lens || (table_width > 0 && !block_table) || (num_pages > 0 && (!k_cache || !v_cache)))
         return fail(MYFA_E_INVALID, "%s: null pointer", what);

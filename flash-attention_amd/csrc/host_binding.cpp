@@ -126,9 +126,10 @@ WindowSizes check_window(const Tensor& q, const Tensor& k, const Tensor& v, py::
     TORCH_CHECK(w.d <= most, what, " supports head dims up to ", most, " for ", q.scalar_type(), ", got ", w.d);
     TORCH_CHECK(w.window >= 1 && w.sinks >= 0, "window must be an integer of at least 1 and sinks one of at least 0, got ", w.window, " and ", w.sinks);
     if (lens.has_value()) check_ints(*lens, {w.B}, q, "seq_lens");
-    // zero columns up to the next head dim whose rows are whole 16-byte chunks change nothing
+    // zero columns up to the next head dim whose rows are whole 16-byte chunks change nothing (no columns at all get some, too:
+    // the logits are 0, and the log-sum-exp is that of as many zeros as a row sees)
     const int64_t step = f32 ? 4 : 8;
-    w.pad = (step - w.d % step) % step;
+    w.pad = w.d == 0 ? step : (step - w.d % step) % step;
     return w;
 }
 
@@ -236,7 +237,7 @@ Cache check_cache(const Tensor& k, const Tensor& v, const Tensor& table, const T
     TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes(), "k_cache and v_cache must be (pages, heads, page, d) tensors of one shape");
     TORCH_CHECK(k.scalar_type() == v.scalar_type(), "Scalar type mismatch!");
     tag(k);
-    TORCH_CHECK(k.size(1) >= 1 && k.size(2) >= 1, "a page holds at least one key of one head");
+    TORCH_CHECK(k.size(1) >= 1 && k.size(2) >= 1 && k.size(3) >= 1, "a page holds at least one key of one head, of at least one column");
     TORCH_CHECK(table.dim() == 2, "block_table must be an int32 (B, width) tensor");
     check_ints(table, table.sizes(), k, "block_table");
     check_ints(lens, {table.size(0)}, k, "seq_lens");

@@ -590,3 +590,12 @@ def test_writes_in_place_are_refused_where_they_cannot_be_made(mfa):
     both = torch.zeros(c.pages, 16, 2, 2, 72, device="cuda", dtype=BF16)[..., :64]
     mfa.paged_kv_append(new, new, both[:, :, 0].transpose(1, 2), both[:, :, 1].transpose(1, 2), table, L)
     assert both.sum() == 2 * 2 * 2 * 64
+
+
+def test_caches_of_no_columns_are_refused(mfa):
+    pool, L, table = torch.zeros(2, 1, 16, 0, device="cuda", dtype=BF16), _i32([3]), _i32([[1]])
+    sums = torch.zeros(1, 1, 16, device="cuda")
+    for call in (lambda: mfa.paged_attn_decode(torch.zeros(1, 1, 0, device="cuda", dtype=BF16), pool, pool, table, L, weight_sum=sums, return_lse=True),
+                 lambda: mfa.paged_kv_append(pool[:1], pool[:1], pool, pool, table, L), lambda: mfa.paged_kv_evict(pool, pool, sums, table, L, table, 4)):
+        with pytest.raises(RuntimeError, match="at least one column"):
+            call()

@@ -211,3 +211,18 @@ for call in (lambda: m.window_attn_fwd(x, x, x, 4), lambda: m.window_attn_func(x
 """ % str(tmp_path)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=tmp_path, env={**os.environ, "PYTHONPATH": str(tmp_path)})
     assert r.returncode == 0, r.stderr
+
+
+def test_head_dim_of_zero():
+    """An output of no elements is written by not launching anything; the other results of such a call are refused."""
+    lib, bf16 = _lib.lib, _lib.MYFA_BF16
+    st = S3(0, 0, 0)
+
+    def fwd(lse):
+        return lib.myfa_window_attn_fwd(16, 16, 16, 16, lse, None, 1, 2, 1, 4, 8, 0, st, st, st, 4, 0, 1.0, bf16, None)
+
+    def decode(lse, sums):
+        return lib.myfa_paged_attn_decode(16, 16, 16, 16, 16, 16, lse, sums, 1, 4, 2, 0, 8, 16, 4, st, st, st, 0, 0, 1.0, bf16, None, 0, None)
+    assert fwd(None) == 0 and decode(None, None) == 0
+    for rc in (fwd(16), decode(16, None), decode(None, 16)):
+        _error(rc, 2, "head dim 0")

@@ -535,3 +535,18 @@ def test_rows_behind_the_length_do_not_change_the_others(mfa, d, dtype):
         cut, cut_lse = mfa.window_attn_fwd(q, k, v, 1024, scale=0.002, return_lse=True, seq_lens=L)
         assert torch.equal(cut[:, :, :n], out[:, :, :n]) and torch.equal(cut_lse[:, :, :n], lse[:, :, :n]), n
         assert not cut[:, :, n:].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_head_dim_of_zero(mfa, dtype):
+    """All logits are 0: the log-sum-exp is the logarithm of how many keys a row sees."""
+    q, k, v, dout = (t.cuda() for t in _inputs(2, 2, 1, 40, 50, 0, dtype))
+    L = torch.tensor([50, 30], dtype=torch.int32, device="cuda")
+    taken = torch.full((2, 2, 40), 7.0, device="cuda")       # (what an allocation of that size holds next)
+    del taken
+    out, lse = mfa.window_attn_fwd(q, k, v, 9, sinks=2, return_lse=True, seq_lens=L)
+    assert out.shape == q.shape
+    want = ref.attention(*(t.cpu() for t in (q, k, v)), _visible(2, 40, 50, 9, 2, [50, 30]), 1.0, dtype)
+    ref.check("lse", lse, want["lse"])
+    for g, t in zip(mfa.window_attn_bwd(dout, q, k, v, out, lse, 9, sinks=2, seq_lens=L), (q, k, v)):
+        assert g.shape == t.shape
