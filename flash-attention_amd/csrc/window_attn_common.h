@@ -33,8 +33,6 @@ constexpr float kLn2W = 0.6931471805599453f;
 constexpr int kOffPast = 0x7FFF0000;
 constexpr int kTileBytesMax = 0x7FFE0000;
 
-__device__ __forceinline__ constexpr int cdiv32(int a, int b) { return (a + b - 1) / b; }
-
 template <typename T> struct Frag16 { using type = s16x8; };
 template <> struct Frag16<float> { using type = f32x4; };
 
