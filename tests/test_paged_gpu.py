@@ -599,3 +599,34 @@ def test_caches_of_no_columns_are_refused(mfa):
                  lambda: mfa.paged_kv_append(pool[:1], pool[:1], pool, pool, table, L), lambda: mfa.paged_kv_evict(pool, pool, sums, table, L, table, 4)):
         with pytest.raises(RuntimeError, match="at least one column"):
             call()
+
+
+def test_results_do_not_depend_on_fresh_memory(mfa):
+    """Outputs and workspaces filled with NaN (whole numbers with their largest) before the call change nothing: torch does that to fresh
+    memory in its deterministic mode."""
+    def calls():
+        for lens, H, G, page, d, window, sinks, width in (([500, 0, 1, 31, 513], 8, 2, 16, 128, 0, 0, None), ([40, 200], 40, 2, 32, 64, 0, 0, 64),
+                                                          ([5000, 40], 4, 1, 32, 80, 700, 4, None), ([3000, 90, 0], 4, 2, 24, 128, 0, 0, 400)):
+            c = Cache(lens, G, page, d, BF16, 16, spare=8 * len(lens), width=width)
+            q = torch.randn(len(lens), H, d, generator=c.gen).to(BF16).cuda()
+            args = c.gpu()
+            sums = torch.rand(len(lens), G, c.width * page, generator=c.gen).cuda()
+            yield mfa.paged_attn_decode(q, *args, scale=0.1, window=window, sinks=sinks, return_lse=True)
+            yield (*mfa.paged_attn_decode(q, *args, scale=0.1, window=window, sinks=sinks, weight_sum=sums, return_lse=True), sums)
+            for budget in (17, 100):
+                new_table = torch.full((len(lens), 8), -1, dtype=torch.int32)
+                for b, n in enumerate(lens):
+                    for j in range(-(-min(n, budget) // page)):
+                        new_table[b, j] = c.free[8 * b + j]
+                yield (*mfa.paged_kv_evict(*args[:2], sums, *args[2:], new_table.cuda(), budget, sinks=2, recent=5), *args[:2])
+    want = [[t.clone() for t in x] for x in calls()]
+    before = torch.are_deterministic_algorithms_enabled(), torch.utils.deterministic.fill_uninitialized_memory
+    try:
+        torch.use_deterministic_algorithms(True, warn_only=True)
+        torch.utils.deterministic.fill_uninitialized_memory = True
+        assert torch.isnan(torch.empty(5, device="cuda")).all()
+        for x, y in zip(calls(), want):
+            assert len(x) == len(y) and all(torch.equal(a.float().nan_to_num(9.0), b.float().nan_to_num(9.0)) for a, b in zip(x, y))
+    finally:
+        torch.use_deterministic_algorithms(before[0])
+        torch.utils.deterministic.fill_uninitialized_memory = before[1]

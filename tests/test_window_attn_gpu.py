@@ -550,3 +550,28 @@ def test_head_dim_of_zero(mfa, dtype):
     ref.check("lse", lse, want["lse"])
     for g, t in zip(mfa.window_attn_bwd(dout, q, k, v, out, lse, 9, sinks=2, seq_lens=L), (q, k, v)):
         assert g.shape == t.shape
+
+
+def test_results_do_not_depend_on_fresh_memory(mfa):
+    """Outputs and workspaces filled with NaN before the call change nothing: torch does that to fresh memory in its deterministic mode."""
+    cases = [(2, 6, 2, 77, 150, 80, 33, 1, [150, 90], BF16), (3, 2, 2, 65, 65, 64, 20, 2, [65, 0, 1], F32), (1, 2, 1, 640, 640, 64, 100, 130, None, F16),
+             (4, 48, 48, 130, 333, 128, 64, 4, [333, 200, 203, 0], BF16), (1, 60, 30, 513, 513, 128, 90, 5, None, F16),
+             (1, 96, 96, 700, 700, 32, 90, 5, None, F32), (2, 72, 72, 140, 140, 192, 50, 3, [140, 90], BF16), (1, 8, 8, 20, 1200, 128, 150, 3, None, BF16),
+             (1, 2, 1, 100, 140, 20, 30, 2, [120], BF16)]
+
+    def calls():
+        for B, H, G, nq, nk, d, window, sinks, lens, dtype in cases:
+            q, k, v, dout = (t.cuda() for t in _inputs(B, H, G, nq, nk, d, dtype, 17))
+            yield _run(mfa, q, k, v, dout, window, sinks, d ** -0.5, lens)
+    want = list(calls())
+    before = torch.are_deterministic_algorithms_enabled(), torch.utils.deterministic.fill_uninitialized_memory
+    try:
+        torch.use_deterministic_algorithms(True, warn_only=True)
+        torch.utils.deterministic.fill_uninitialized_memory = True
+        assert torch.isnan(torch.empty(5, device="cuda")).all()
+        for x, y in zip(calls(), want):
+            for name in x:
+                assert torch.equal(x[name], y[name]), name
+    finally:
+        torch.use_deterministic_algorithms(before[0])
+        torch.utils.deterministic.fill_uninitialized_memory = before[1]
