@@ -9,14 +9,19 @@
 //   S^T[32 keys x 16 heads] = K Q^T on v_mfma 16x16 (16x16x32 16-bit, 16x16x4 float32), K chunks straight from
 //   memory to registers as the A operand; running maximum and sum per head (float32, base 2); P^T is in place
 //   the B operand of O^T[d x 16 heads] += V^T P^T, V^T coming through a wave-private LDS tile by transposing
-//   reads.  The next tile's K and V are requested before the exponentials of this one.
+//   reads.  P is rounded to the element type there (the matrix cores take operands of one type, and 16-bit ones at sixteen
+//   times float32's rate); logits, maxima, sums, parts and the weights that are added up are float32.
+//   The next tile's K and V are requested before the exponentials of this one.
 // The waves of a workgroup are joined through LDS; with more than one share per head a second launch joins the
 // shares' unnormalised sums, in order.  With `weight_sum`, the logits are kept in the workspace (4 bytes per
 // head and key against 4 d read) and the second launch adds exp(logit - lse), summed over the group's heads in
 // order, to the running sum of each key.
-// Measured, 32 heads on 8, d 128: 8 sequences of up to 131072 keys (f16, 2.7 GB) 476 us = 5.76 TB/s, what a sum over a large
-// tensor reaches; 64 of up to 4096 with weights (bf16, 615 MB) 157 us = 3.9 TB/s, of which the join and the weights take
-// 13; one sequence of 1024 keys 12.3 us: two launches, 9.4 us of dependent loads (table, keys, values) and 2.5 us of join.
+// Measured, 32 heads on 8, d 128: 8 sequences of up to 131072 keys (f16, 2.7 GB) 476 us = 5.76 TB/s, where a
+// product of a matrix and a vector of that size reaches 6.1; 64 of up to 4096 with weights (bf16, 615 MB) 157 us = 3.9 TB/s.  There
+// the weights are 20 of it (and the join's launch 13), and unequal lengths little: all of one length 155, sorted 148.  The rest
+// is that shares are short: a wave has four tiles in the longest sequence and one or none in a short one, and its first loads and the
+// joins in LDS and memory stand beside them.  One sequence of 1024 keys 12.1 us: two launches, 9.4 us of dependent loads (table,
+// keys, values) and 2.5 us of join.
 // Append: 64 tokens 4.2 us (a launch); 8 prompts of 4096 (268 MB) 55 us = 4.9 TB/s.
 #include "paged_common.h"
 

@@ -4,7 +4,10 @@
 // sees would reach the others of its tile.  Nothing in the loops looks for that.  Where at the end a wave's float32 sums
 // are not finite, it looks through what its tiles held hidden (the tiles at the edges of what its rows see, no more) for
 // columns that are not finite; in those alone its rows are formed again, key by key (or its keys query by query) over
-// what they see and nothing else, with the columns on the lanes and until nothing finite is left in them.
+// what they see and nothing else, with the columns on the lanes and until nothing finite is left in them (a column that is infinite
+// by then stays so, though a later key would make it NaN: which of the two a row gets that sees both infinities is not pinned).
+// The forward looks at hidden values, dQ at hidden keys (hidden values reach hidden dS alone, which are set to 0 behind
+// them), dK and dV at hidden queries, output gradients and statistics.
 // In the ordinary case it is a ballot per 32 rows, which costs nothing that shows: 452 us for 16 heads of 16384 positions with
 // a window of 4096, with and without.  There, a value row of infinities halfway takes the forward to 22 ms and the backward to
 // 176 (one wave forms 32 rows of 4096 keys); one that every later row sees costs the look, 0.7 and 9.5 ms.

@@ -292,7 +292,8 @@ int myfa_matmul_f32(const float* a, const float* b, float* c, int64_t m, int64_t
  * Element types: MYFA_F16 and MYFA_BF16 with d a multiple of 8 up to 256, MYFA_F32 with d a multiple of 4 up to
  * 128; otherwise MYFA_E_UNSUPPORTED.  (d = 0: nothing is written; with lse MYFA_E_UNSUPPORTED.)  Statistics and sums are float32; P is rounded to the element type.
  * What a row does not see, what stands behind a sequence's length included, does not reach it, whatever its bits
- * are.  (Infinities and NaN that some rows see and their neighbours do not cost time: such rows are computed again.)
+ * are.  (Infinities and NaN that some rows see and their neighbours do not cost time: such rows are computed again.  Where what a
+ * row sees itself makes a column not finite, it is not finite; whether infinite or NaN is left open.)
  * No counterpart in the reference, whose attention is unmasked (csrc/api.cpp:168-192).
  */
 int myfa_window_attn_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* seq_lens,
